@@ -112,6 +112,99 @@ PLAMO_API int plamo_k_attention_static(const uint16_t* q, const uint16_t* keys, 
  * CPU restatement reproduces it exactly. n floats, device pointers. */
 PLAMO_API int plamo_k_exp(const float* x, float* y, long long n, void* stream);
 
+/* ---- A serving step over a paged key-value cache -------------------------------------------------
+ * No counterpart in the reference, whose caches are one contiguous slab per lane (Batch.swift:33-78).
+ * One step of a changing set of requests is
+ *     plamo_k_paged_plan -> per layer: plamo_k_paged_qkv, plamo_k_paged_attention -> plamo_k_sample
+ * All four enqueue on `stream`, allocate nothing, keep nothing between calls and can be captured in a
+ * CUDA graph. Values are bf16 (dtype 0) or fp16 (dtype 1) bit patterns. */
+
+/* One layer's paged cache. The value of token slot t = page * page_size + offset, KV head h, element d
+ * is at keys[page * page_stride + offset * token_stride + h * head_stride + d] (values alike); strides in
+ * elements, multiples of 8, keys and values 16-byte aligned. head_dim 64 or 128; page_size >= 1. */
+typedef struct plamo_paged_cache {
+    void* keys;
+    void* values;
+    int32_t dtype;
+    int32_t pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+} plamo_paged_cache;
+
+/* Block table and slot map of one step, from the requests' lengths, on the device. Request r (of rows,
+ * 1...8192) holds the first ceil(lens[r] / page_size) entries of its row of table [rows][table_stride].
+ *   append[r] >= 0: the step appends that many tokens to it; append[r] < 0: the request has ended.
+ * Ended requests' pages go onto the end of free_list (capacity `pages` entries, the first *free_count of
+ * them valid), in request order; the pages the appended tokens need then come off its end, in request
+ * order, as long as they last: a request is refused (nothing granted, nothing appended) when the pages
+ * needed up to and including it exceed the free ones, when it would outgrow its table row, or when its
+ * tokens pass the `tokens` capacity. Outputs: the granted pages in table; new_lens[r] (0 for an ended
+ * request, unchanged for a refused one); row_start[0..rows], the running sums of the appended counts (the
+ * step's tokens are packed in request order); for each of `tokens` packed tokens its position and its slot
+ * (page * page_size + offset), both -1 for a refused request's tokens and past the last token; counts[4]:
+ * free pages left (the next step's free_count), tokens, pages granted, requests refused. An ended
+ * request's table row is left as it was. Entries outside [0, pages) give slot -1. Outputs must not overlap
+ * inputs, except that table and free_list are updated in place. All values int32. */
+PLAMO_API int plamo_k_paged_plan(const int32_t* lens, const int32_t* append, int rows, int page_size, int pages,
+                                 int32_t* table, int table_stride, int32_t* free_list, const int32_t* free_count,
+                                 int32_t* new_lens, int32_t* row_start, int32_t* slots, int32_t* positions, int tokens,
+                                 int32_t* counts, void* stream);
+
+/* QK-norm, rotary embedding and cache append of `tokens` rows of a q/k/v projection, as the forward's own
+ * (Kernels.metal:223-274) but in fp32 with one rounding at the end: a row of qkv (qkv_stride elements
+ * apart) holds heads + 2 * kv_heads heads of head_dim; query and key heads become
+ *   x * rsqrt(mean(x^2) + eps) * (1 + w)   (w = q_norm / k_norm, [head_dim]; NULL: no norm)
+ * and are rotated (rotate-half) by the row of rope [rope_rows][head_dim / 2] at the token's position (u32 =
+ * bf16 cos bits | sin bits << 16; NULL: no rotation, positions unused). Queries go to q (q_stride elements
+ * apart), keys and values to the cache's slot slots[t]. A token whose slot is outside the cache or whose
+ * position is outside rope is not appended and its query row is zero. Two tokens must not share a slot.
+ * Pointers 16-byte aligned, strides multiples of 8. */
+PLAMO_API int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv, int64_t qkv_stride, int tokens, int heads,
+                                const void* q_norm, const void* k_norm, float eps, const uint32_t* rope, int rope_rows,
+                                const int32_t* positions, const int32_t* slots, void* q, int64_t q_stride, void* stream);
+
+/* Attention of one new token of every request over its pages. Request r (of rows, 1...8192) sees the keys
+ * at positions [max(0, n - window), n), n = min(lens[r], max_len) (window 0: all of them); the key at
+ * position p is in page table[r][p / page_size]; entries outside [0, pages) hold no keys (a page given up
+ * behind the window). max_len bounds the lengths for the launch: at most table_stride * page_size.
+ * row_start NULL: request r's query is row r of q [q_rows][heads][head_dim] (q_stride elements apart), and
+ * q_rows >= rows. Else it is row row_start[r + 1] - 1 (the request's last packed token of
+ * plamo_k_paged_plan), and requests without a token are skipped. heads: a multiple of kv_heads, at most 256.
+ *   out = sum_j softmax_j(scale * q.k_j) v_j in fp32 (the probabilities enter the products as hi + lo pairs
+ *   of the 16-bit type), rounded once; lse (may be NULL, [q_rows][heads] fp32) = ln sum_j exp(scale * q.k_j).
+ * A request that sees no key, or whose scores are all -inf, gets zeros and lse -inf. Query rows that belong
+ * to no request are not written. `workspace`: 16-byte aligned device memory of at least
+ * plamo_k_paged_attention_workspace() bytes, no initial contents needed; calls that share one must not
+ * overlap. Pointers 16-byte aligned, strides multiples of 8. */
+PLAMO_API int plamo_k_paged_attention(const plamo_paged_cache* cache, const void* q, int64_t q_stride, int q_rows, int heads,
+                                      const int32_t* table, int table_stride, const int32_t* lens, int rows,
+                                      const int32_t* row_start, int max_len, int window, float scale, void* out,
+                                      int64_t out_stride, float* lse, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* Bytes of workspace that every plamo_k_paged_attention call accepts (no device needed). */
+PLAMO_API size_t plamo_k_paged_attention_workspace(void);
+
+/* Samples one id per row of logits [rows][vocab] (row_stride elements apart; dtype 0 bf16, 1 fp16, 2 fp32;
+ * vocab <= 2^22) by per-row controls on the device (each array NULL: that control off for every row):
+ *   temperature > 0; <= 0 or NaN: greedy (the lowest index of the largest logit). NULL: 1
+ *   top_k > 0: only the top_k largest logits. top_p < 1: only the shortest run of them, in descending
+ *   order, that holds at least top_p of their probability (to 2^-24; never empty). min_p > 0: only ids at
+ *   least min_p times as likely as the most likely one. Ties go to the lower index.
+ * A probability is a whole number w = floor(2^40 * exp((logit - max) / temperature)) (the fp32 exponential),
+ * so every sum is exact and the id does not depend on how the work is split. With u[row] in [0, 1) the
+ * id is the lowest kept index at which the running sum of kept w exceeds floor(2^24 u) * W / 2^24, W the
+ * sum of all kept w. ids[row]; logprobs[row] (may be NULL) = ln(w_id / W); kept[row] (may be NULL) the number
+ * of kept ids. NaN and -inf logits are never chosen; a row of only those gives id 0, logprob -inf and kept 0.
+ * Equal +inf logits share the probability. */
+PLAMO_API int plamo_k_sample(const void* logits, int dtype, int rows, int vocab, int64_t row_stride,
+                             const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                             const float* u, int32_t* ids, float* logprobs, int32_t* kept, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,6 +119,15 @@ def library() -> ctypes.CDLL:
                                                   ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_size_t,
                                                   _vp]),
         "plamo_k_exp": (ctypes.c_int, [_vp, _vp, ctypes.c_longlong, _vp]),
+        "plamo_k_paged_plan": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int] +
+                               [_vp] * 6 + [ctypes.c_int, _vp, _vp]),
+        "plamo_k_paged_qkv": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp, _vp,
+                                             ctypes.c_float, _vp, ctypes.c_int, _vp, _vp, _vp, ctypes.c_int64, _vp]),
+        "plamo_k_paged_attention": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int,
+                                                   _vp, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_float,
+                                                   _vp, ctypes.c_int64, _vp, _vp, ctypes.c_size_t, _vp]),
+        "plamo_k_paged_attention_workspace": (ctypes.c_size_t, []),
+        "plamo_k_sample": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64] + [_vp] * 9),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -493,3 +502,45 @@ def k_attention_rows(q, keys, values, heads, kv_heads, cap, geo, rows, full, rop
 
 def k_exp(x, y, n, stream=0):
     _check(library().plamo_k_exp(x, y, int(n), stream or None))
+
+
+class PagedCache(ctypes.Structure):
+    """One layer's paged key-value cache (plamo_paged_cache): device pointers, dtype (0 bf16, 1 fp16), geometry
+    and element strides. Made once beside the cache's memory; k_paged_qkv and k_paged_attention take it."""
+    _fields_ = [("keys", _vp), ("values", _vp)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "pages", "page_size", "kv_heads", "head_dim")] + \
+               [(n, ctypes.c_int64) for n in ("page_stride", "token_stride", "head_stride")]
+
+
+def k_paged_plan(lens, append, rows, page_size, pages, table, table_stride, free_list, free_count, new_lens, row_start,
+                 slots, positions, tokens, counts, stream=0):
+    """plamo_k_paged_plan: block table, slot map and positions of one step from the requests' lengths."""
+    _check(library().plamo_k_paged_plan(lens, append, rows, page_size, pages, table, table_stride, free_list, free_count,
+                                        new_lens, row_start, slots, positions, tokens, counts, stream or None))
+
+
+def k_paged_qkv(cache, qkv, qkv_stride, tokens, heads, q_norm, k_norm, eps, rope, rope_rows, positions, slots, q, q_stride,
+                stream=0):
+    """plamo_k_paged_qkv: QK-norm, rotary embedding and append of the step's tokens to the paged cache."""
+    _check(library().plamo_k_paged_qkv(ctypes.addressof(cache), qkv, qkv_stride, tokens, heads, q_norm or None,
+                                       k_norm or None, eps, rope or None, rope_rows, positions or None, slots, q, q_stride,
+                                       stream or None))
+
+
+def k_paged_attention(cache, q, q_stride, q_rows, heads, table, table_stride, lens, rows, row_start, max_len, window, scale,
+                      out, out_stride, lse, workspace, workspace_bytes, stream=0):
+    """plamo_k_paged_attention: one new token of every request over its pages."""
+    _check(library().plamo_k_paged_attention(ctypes.addressof(cache), q, q_stride, q_rows, heads, table, table_stride, lens,
+                                             rows, row_start or None, max_len, window, scale, out, out_stride, lse or None,
+                                             workspace, workspace_bytes, stream or None))
+
+
+def paged_attention_workspace() -> int:
+    """Bytes of workspace that every k_paged_attention call accepts."""
+    return library().plamo_k_paged_attention_workspace()
+
+
+def k_sample(logits, dtype, rows, vocab, row_stride, temperature, top_k, top_p, min_p, u, ids, logprobs=0, kept=0, stream=0):
+    """plamo_k_sample: one id per row by temperature, top-k, top-p and min-p from given uniform numbers."""
+    _check(library().plamo_k_sample(logits, dtype, rows, vocab, row_stride, temperature or None, top_k or None, top_p or None,
+                                    min_p or None, u, ids, logprobs or None, kept or None, stream or None))
