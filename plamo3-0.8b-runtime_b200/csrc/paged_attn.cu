@@ -3,17 +3,27 @@
 //   s_j = scale * q.k_j;  o = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m};  lse = m + ln sum_j e^{s_j - m}
 // in one pass over the keys with a running maximum and sum. Scores are kept in powers of two.
 //
-// A block takes one request and one KV head (at most 16 of its query heads: the rows of an m16n8k16 MMA;
-// a larger group takes several blocks). Its four warps take every fourth 16-key tile, each with its own
-// maximum, sum and output accumulators, and are joined in shared memory at the end. A tile's keys and
-// values are copied with cp.async in an XOR-swizzled layout, so ldmatrix reads them without bank
-// conflicts. Keys outside the visible range or without a page are filled with zeros and their scores
-// replaced by -inf, so nothing stored there can reach a result.
+// Split. The work is a line of units (64 keys of one request and one KV head, at most 16 of its query
+// heads: the rows of an m16n8k16 MMA), request after request. Each block takes one stretch of equal length
+// of that line, whatever the lengths are, so a batch of any raggedness ends in one wave. The lengths are
+// on the device: every block adds them up itself. A request and head inside one stretch is finished there;
+// one that is cut leaves an fp32 partial per block, and k_paged_join adds those up in order, so a
+// result does not depend on timing. Calls whose requests cannot be cut launch no join.
+//
+// Block. Four warps take every fourth 16-key tile of a stretch, each with its own running maximum, sum and
+// outputs and its own ring of tiles: no barrier inside the loop. A tile's keys and values are copied with
+// cp.async in an XOR-swizzled layout, so ldmatrix reads them without bank conflicts; the page lookup of a
+// tile runs one tile ahead of its copy. Keys outside the visible range or without a page are filled
+// with zeros and their scores replaced by -inf, so nothing stored there can reach a result.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "paged.h"
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
 
 namespace plamo {
 namespace {
@@ -22,6 +32,14 @@ constexpr int PA_THREADS = 128;
 constexpr int PA_WARPS = PA_THREADS / 32;
 constexpr int PA_HEADS = 16;  // query heads of a block: the MMA's rows
 constexpr int PA_TILE = 16;   // keys of a tile
+constexpr int PA_UNIT = 64;   // keys of a unit: one tile for each warp
+// Requests of at most this many keys are one unit and never cut.
+constexpr int PA_WHOLE = 256;
+constexpr int PA_MAX_BLOCKS = 592;
+constexpr int JOIN_THREADS = 256;
+// tiles in a warp's ring: 96 KB a block, two blocks an SM
+template <int D>
+constexpr int PA_STAGES = 384 / D;
 
 template <bool HALF>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -160,108 +178,363 @@ __device__ __forceinline__ void add_tile(Running<D>& run, const uint32_t (&qa)[D
     }
 }
 
-template <int D, bool HALF>
-__global__ void __launch_bounds__(PA_THREADS) k_paged_attn(PagedAttnArgs a, int group, int blocks_per_kv) {
-    constexpr int ROW = D * 2, TILE_BYTES = PA_TILE * ROW, CH = D / 8;
-    // the warps' tiles; afterwards the warps' outputs
-    __shared__ __align__(128) uint8_t smem[PA_WARPS * PA_HEADS * D * 4];
-    __shared__ float2 stats[PA_WARPS][PA_HEADS];
-    static_assert(PA_WARPS * 2 * TILE_BYTES <= int(sizeof(smem)), "tiles fit");
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gq = lane >> 2, tq = lane & 3;
-    const int r = blockIdx.y, kv = blockIdx.x / blocks_per_kv, h0 = (blockIdx.x % blocks_per_kv) * PA_HEADS;
-    int qrow = r;
+// Four finished outputs of a head, and its lse.
+template <bool HALF>
+__device__ __forceinline__ void store_row(const PagedAttnArgs& a, int qrow, int head, int D, int d, float4 o, float m, float l) {
+    const float inv = 1.0f / (l > 0.f ? l * P_PAIR : 1.f);
+    uint2 w;
+    w.x = round16<HALF>(o.x * inv) | uint32_t(round16<HALF>(o.y * inv)) << 16;
+    w.y = round16<HALF>(o.z * inv) | uint32_t(round16<HALF>(o.w * inv)) << 16;
+    *reinterpret_cast<uint2*>(a.out + qrow * a.out_stride + head * D + d) = w;
+    if (a.lse && d == 0) a.lse[size_t(qrow) * a.heads + head] = (origin(m) - P_SHIFT<HALF> + log2f(l)) * 0.693147180559945309f;
+}
+
+int sm_count() {
+    static const int n = [] {
+        int dev = 0, v = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) v = 148;
+        return std::min(v, PA_MAX_BLOCKS / 2);
+    }();
+    return n;
+}
+
+// What k_paged_join needs of one cut request and head: its query row (-1: nothing to join), heads, the blocks
+// first_block ... first_block + pieces - 1 that hold a piece, and the first one's place.
+struct __align__(16) JoinRecord {
+    int qrow, head0, heads, pieces;
+    int first_slot, first_block, pad0, pad1;
+};
+// Workspace: records, then 2 partials a block (the stretch's first and its last request), each 16 heads x
+// head_dim outputs, then 2 x 16 (maximum, sum) pairs a block.
+constexpr size_t PA_PART_AT = size_t(PA_MAX_BLOCKS) * sizeof(JoinRecord);
+constexpr size_t PA_STATS_AT = PA_PART_AT + size_t(2) * PA_MAX_BLOCKS * PA_HEADS * 128 * sizeof(float);
+constexpr size_t PA_WORKSPACE = PA_STATS_AT + size_t(2) * PA_MAX_BLOCKS * PA_HEADS * sizeof(float2);
+
+struct Split {
+    int unit;       // keys of a unit
+    int pairs;      // (KV head, block of 16 query heads) pairs of a request
+    int per_kv;     // blocks of 16 query heads of a KV head
+    int by_pair;    // join records are indexed by (request, pair), else by block
+    int join;       // a join follows
+};
+
+// The query row of request r, -1 when it has none.
+__device__ __forceinline__ int query_row(const PagedAttnArgs& a, int r) {
+    int q = r;
     if (a.row_start) {
-        const int next = a.row_start[r + 1];
-        if (next <= a.row_start[r]) return;
-        qrow = next - 1;
+        q = a.row_start[r + 1] - 1;
+        if (q < a.row_start[r]) return -1;
     }
-    if (qrow < 0 || qrow >= a.q_rows) return;
-    const int heads = min(PA_HEADS, group - h0), head0 = kv * group + h0;
-    const int n = min(max(a.lens[r], 0), a.max_len), first = a.window > 0 ? max(0, n - a.window) : 0;
-    uint32_t qa[D / 16][4];
-    const uint16_t* q = a.q + qrow * a.q_stride + head0 * D;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; kk++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int h = gq + (i & 1) * 8, d = kk * 16 + 2 * tq + (i >> 1) * 8;
-            qa[kk][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + h * D + d) : 0u;
+    return q >= 0 && q < a.q_rows ? q : -1;
+}
+
+template <int D, bool HALF>
+__global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, Split sp) {
+    pdl_enter();
+    constexpr int ROW = D * 2, TILE_BYTES = PA_TILE * ROW, CH = D / 8, S = PA_STAGES<D>;
+    extern __shared__ __align__(128) uint8_t pa_smem[];
+    // the warps' rings, afterwards the warps' outputs; then the running sums of the requests' units
+    constexpr int RING_BYTES = PA_WARPS * S * 2 * TILE_BYTES;
+    static_assert(PA_WARPS * PA_HEADS * D * 4 <= RING_BYTES, "the outputs fit in the rings");
+    int* const upto = reinterpret_cast<int*>(pa_smem + RING_BYTES);  // [rows + 1]
+    __shared__ float2 stats[PA_WARPS][PA_HEADS];
+    __shared__ int warp_sums[PA_WARPS];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gq = lane >> 2, tq = lane & 3;
+    JoinRecord* const records = static_cast<JoinRecord*>(a.workspace);
+    float* const parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + PA_PART_AT);
+    float2* const part_stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.workspace) + PA_STATS_AT);
+
+    // running sums of the units
+    {
+        const int per = (a.rows + PA_THREADS - 1) / PA_THREADS, r0 = min(t * per, a.rows), r1 = min(r0 + per, a.rows);
+        int sum = 0;
+        for (int r = r0; r < r1; r++) {
+            const int n = min(max(a.lens[r], 0), a.max_len), seen = a.window > 0 ? min(n, a.window) : n;
+            const int units = query_row(a, r) >= 0 ? (seen + sp.unit - 1) / sp.unit : 0;
+            upto[r + 1] = units;
+            sum += units;
         }
-    Running<D> run;
-    run.clear();
-    const uint32_t kt = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
-    const int* table = a.table + size_t(r) * a.table_stride;
-    for (int k0 = first + warp * PA_TILE; k0 < n; k0 += PA_WARPS * PA_TILE) {
-        // lane j < 16 finds key j; the row's chunks are then copied by 16 (D = 128) or 8 lanes each
-        long long at = -1;
-        const int key = k0 + (lane & 15);
-        if (key < n) {
-            const int slot = key / a.cache.page_size, page = table[slot];
+        int x = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(FULL_MASK, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) warp_sums[warp] = x;
+        __syncthreads();
+        int at = x - sum;
+        for (int w = 0; w < warp; w++) at += warp_sums[w];
+        for (int r = r0; r < r1; r++) {
+            at += upto[r + 1];
+            upto[r + 1] = at;
+        }
+        if (t == 0) upto[0] = 0;
+        __syncthreads();
+    }
+    const long long total = (long long)upto[a.rows] * sp.pairs;
+    const long long per_block = max((total + gridDim.x - 1) / gridDim.x, 1ll);
+    const long long x0 = min(blockIdx.x * per_block, total), x1 = min(x0 + per_block, total);
+
+    // requests that see nothing
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        if (upto[r + 1] != upto[r]) continue;
+        if (sp.join && sp.by_pair)
+            for (int p = t; p < sp.pairs; p += PA_THREADS) records[r * sp.pairs + p].qrow = -1;
+        const int qrow = query_row(a, r);
+        if (qrow < 0) continue;
+        for (int i = t; i < a.heads * D; i += PA_THREADS) a.out[qrow * a.out_stride + i] = 0;
+        if (a.lse)
+            for (int h = t; h < a.heads; h += PA_THREADS) a.lse[size_t(qrow) * a.heads + h] = -INFINITY;
+    }
+    if (sp.join && !sp.by_pair && t == 0) {
+        // record of this block: the request and head that reach into its stretch from the block before,
+        // when no earlier block begins inside them (written below once they are known)
+        if (x0 >= x1) records[blockIdx.x].qrow = -1;
+    }
+
+    const int group = a.heads / a.cache.kv_heads;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(pa_smem)) + warp * S * 2 * TILE_BYTES;
+    for (long long x = x0; x < x1;) {
+        // the request of unit x: the last one whose units begin at or before it
+        int lo = 0, hi = a.rows - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if ((long long)upto[mid] * sp.pairs <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        const int r = lo, units = upto[r + 1] - upto[r];
+        const long long inside = x - (long long)upto[r] * sp.pairs;
+        const int pair = int(inside / units), u = int(inside - (long long)pair * units);
+        const int take = int(min((long long)(units - u), x1 - x));
+        const int kv = pair / sp.per_kv, h0 = (pair % sp.per_kv) * PA_HEADS;
+        const int heads = min(PA_HEADS, group - h0), head0 = kv * group + h0;
+        const int qrow = query_row(a, r);
+        const int n = min(max(a.lens[r], 0), a.max_len), first = a.window > 0 ? max(0, n - a.window) : 0;
+        const int k0 = first + u * sp.unit, k1 = min((long long)n, k0 + (long long)take * sp.unit);
+        const bool whole = take == units;
+        if (sp.join && t == 0) {
+            const long long begin = x - u;  // the pair's first unit on the line
+            const int b0 = int(begin / per_block), b1 = int((begin + units - 1) / per_block);
+            const JoinRecord rec{b1 > b0 ? qrow : -1, head0, heads, b1 - b0 + 1, 2 * b0 + (begin != b0 * per_block), b0, 0, 0};
+            if (sp.by_pair) {
+                if (u == 0) records[r * sp.pairs + pair] = rec;
+            } else if (x == x0) {
+                records[blockIdx.x] = rec;
+                if (u == 0 || (int)blockIdx.x != b0 + 1) records[blockIdx.x].qrow = -1;
+            }
+        }
+        // queries: rows gq and gq + 8 of the MMA
+        uint32_t qa[D / 16][4];
+        const uint16_t* q = a.q + qrow * a.q_stride + head0 * D;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; kk++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int h = gq + (i & 1) * 8, d = kk * 16 + 2 * tq + (i >> 1) * 8;
+                qa[kk][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + h * D + d) : 0u;
+            }
+        Running<D> run;
+        run.clear();
+        const int* table = a.table + size_t(r) * a.table_stride;
+        const int tiles = (k1 - k0 + PA_TILE - 1) / PA_TILE;
+        const int mine = tiles > warp ? (tiles - warp + PA_WARPS - 1) / PA_WARPS : 0;
+        // lane j < 16 (and j + 16) looks up key j of a tile: its page, -1 outside the range
+        auto page_of = [&](int j) -> int {
+            const int key = k0 + (warp + j * PA_WARPS) * PA_TILE + (lane & 15);
+            return j < mine && key < k1 ? __ldg(table + key / a.cache.page_size) : -1;
+        };
+        auto issue = [&](int j, int page) -> uint32_t {
+            const int key = k0 + (warp + j * PA_WARPS) * PA_TILE + (lane & 15);
+            long long at = -1;
             if (page >= 0 && page < a.cache.pages)
-                at = page * a.cache.page_stride + (key - slot * a.cache.page_size) * a.cache.token_stride +
-                     kv * a.cache.head_stride;
-        }
-        const uint32_t mask = __ballot_sync(FULL_MASK, at >= 0) & 0xffffu;
+                at = page * a.cache.page_stride + (key % a.cache.page_size) * a.cache.token_stride + kv * a.cache.head_stride;
+            const uint32_t mask = __ballot_sync(FULL_MASK, at >= 0) & 0xffffu;
+            const uint32_t kt = ring + (j % S) * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
 #pragma unroll
-        for (int i = 0; i < PA_TILE * CH / 32; i++) {
-            const int row = i * (32 / CH) + lane / CH, c = lane % CH;
-            const long long off = __shfl_sync(FULL_MASK, at, row);
-            const uint32_t dst = row * ROW + ((c ^ (row & 7)) << 4);
-            copy16(kt + dst, a.cache.keys + max(off, 0ll) + c * 8, off >= 0);
-            copy16(vt + dst, a.cache.values + max(off, 0ll) + c * 8, off >= 0);
-        }
-        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
-        __syncwarp();
-        add_tile<D, HALF>(run, qa, kt, vt, mask, a.scale_log2);
-        __syncwarp();
-    }
-    // join the warps
+            for (int i = 0; i < PA_TILE * CH / 32; i++) {
+                const int row = i * (32 / CH) + lane / CH, c = lane % CH;
+                const long long off = __shfl_sync(FULL_MASK, at, row);
+                const uint32_t dst = row * ROW + ((c ^ (row & 7)) << 4);
+                copy16(kt + dst, a.cache.keys + max(off, 0ll) + c * 8, off >= 0);
+                copy16(vt + dst, a.cache.values + max(off, 0ll) + c * 8, off >= 0);
+            }
+            return mask;
+        };
+        uint32_t masks[S];  // of the tiles in flight, oldest first
+        int next = page_of(0);
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 1);
-        run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 2);
-        if (tq == 0) stats[warp][gq + 8 * h] = make_float2(run.m[h], run.l[h]);
+        for (int s = 0; s < S - 1; s++) {
+            const int page = next;
+            next = page_of(s + 1);
+            masks[s] = s < mine ? issue(s, page) : 0u;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        for (int j = 0; j < mine; j++) {
+            const int page = next;
+            next = page_of(j + S);
+            masks[S - 1] = j + S - 1 < mine ? issue(j + S - 1, page) : 0u;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+            __syncwarp();
+            const uint32_t kt = ring + (j % S) * 2 * TILE_BYTES;
+            add_tile<D, HALF>(run, qa, kt, kt + TILE_BYTES, masks[0], a.scale_log2);
+            __syncwarp();  // the tile has been read: the next copy may overwrite it
+#pragma unroll
+            for (int s = 0; s < S - 1; s++) masks[s] = masks[s + 1];
+        }
+        // join the warps
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 1);
+            run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 2);
+            if (tq == 0) stats[warp][gq + 8 * h] = make_float2(run.m[h], run.l[h]);
+        }
+        __syncthreads();  // every warp is done with its ring
+        float* const mid = reinterpret_cast<float*>(pa_smem);
+#pragma unroll
+        for (int j = 0; j < D / 8; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                *reinterpret_cast<float2*>(mid + (warp * PA_HEADS + gq + 8 * h) * D + j * 8 + 2 * tq) =
+                    make_float2(run.o[j][2 * h], run.o[j][2 * h + 1]);
+        __syncthreads();
+        const int slot = 2 * blockIdx.x + (x != x0);
+        for (int i = t; i < heads * (D / 4); i += PA_THREADS) {
+            const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][h].x);
+            float l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; w++) {
+                const float f = ex2(stats[w][h].x - origin(m));
+                const float4 v = *reinterpret_cast<const float4*>(mid + (w * PA_HEADS + h) * D + d);
+                l = fmaf(stats[w][h].y, f, l);
+                o.x = fmaf(v.x, f, o.x);
+                o.y = fmaf(v.y, f, o.y);
+                o.z = fmaf(v.z, f, o.z);
+                o.w = fmaf(v.w, f, o.w);
+            }
+            if (whole) {
+                store_row<HALF>(a, qrow, head0 + h, D, d, o, m, l);
+            } else {
+                *reinterpret_cast<float4*>(parts + (size_t(slot) * PA_HEADS + h) * D + d) = o;
+                if (d == 0) part_stats[slot * PA_HEADS + h] = make_float2(m, l);
+            }
+        }
+        __syncthreads();  // the rings and stats are free again
+        x += take;
     }
+}
+
+// Adds up the pieces of one head of a cut request: warp w takes every eighth piece, then the warps are added.
+template <int D, bool HALF>
+__global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a) {
+    pdl_enter();
+    constexpr int WARPS = JOIN_THREADS / 32, VEC = D / 32;
+    __shared__ float outs[WARPS][D];
+    __shared__ float2 stats[WARPS];
+    const JoinRecord rec = static_cast<const JoinRecord*>(a.workspace)[blockIdx.x];
+    const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (rec.qrow < 0 || h >= rec.heads) return;
+    const float* const parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + PA_PART_AT);
+    const float2* const part_stats = reinterpret_cast<const float2*>(static_cast<const uint8_t*>(a.workspace) + PA_STATS_AT);
+    float m = -INFINITY, l = 0.f, o[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; i++) o[i] = 0.f;
+    constexpr int BATCH = 4;  // pieces whose reads are in flight together
+    for (int p0 = warp; p0 < rec.pieces; p0 += WARPS * BATCH) {
+        float2 st[BATCH];
+        float v[BATCH][VEC];
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+            const int p = p0 + b * WARPS, slot = p == 0 ? rec.first_slot : 2 * (rec.first_block + p);
+            st[b] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) v[b][i] = 0.f;
+            if (p < rec.pieces) {
+                st[b] = part_stats[slot * PA_HEADS + h];
+                const float* src = parts + (size_t(slot) * PA_HEADS + h) * D + lane * VEC;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) v[b][i] = src[i];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+            const float top = fmaxf(m, st[b].x), fade = ex2(m - origin(top)), f = ex2(st[b].x - origin(top));
+            l = fmaf(st[b].y, f, l * fade);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o[i] = fmaf(v[b][i], f, o[i] * fade);
+            m = top;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; i++) outs[warp][lane * VEC + i] = o[i];
+    if (lane == 0) stats[warp] = make_float2(m, l);
     __syncthreads();
-    float* const part = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int j = 0; j < D / 8; j++)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            *reinterpret_cast<float2*>(part + (warp * PA_HEADS + gq + 8 * h) * D + j * 8 + 2 * tq) =
-                make_float2(run.o[j][2 * h], run.o[j][2 * h + 1]);
-    __syncthreads();
-    for (int i = t; i < heads * D; i += PA_THREADS) {
-        const int h = i / D;
-        float m = -INFINITY;
-        for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][h].x);
-        float l = 0.f, o = 0.f;
-        for (int w = 0; w < PA_WARPS; w++) {
-            const float f = ex2(stats[w][h].x - origin(m));
-            l = fmaf(stats[w][h].y, f, l);
-            o = fmaf(part[(w * PA_HEADS + h) * D + i % D], f, o);
-        }
-        a.out[qrow * a.out_stride + head0 * D + i] = round16<HALF>(o / (l > 0.f ? l * P_PAIR : 1.f));
-        if (a.lse && i % D == 0)
-            a.lse[size_t(qrow) * a.heads + head0 + h] = (origin(m) - P_SHIFT<HALF> + log2f(l)) * 0.693147180559945309f;
+    if (threadIdx.x >= D / 4) return;
+    const int d = threadIdx.x * 4;
+    float top = -INFINITY, sum = 0.f;
+    for (int w = 0; w < WARPS; w++) top = fmaxf(top, stats[w].x);
+    float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < WARPS; w++) {
+        const float f = ex2(stats[w].x - origin(top));
+        const float4 v = *reinterpret_cast<const float4*>(&outs[w][d]);
+        sum = fmaf(stats[w].y, f, sum);
+        out.x = fmaf(v.x, f, out.x);
+        out.y = fmaf(v.y, f, out.y);
+        out.z = fmaf(v.z, f, out.z);
+        out.w = fmaf(v.w, f, out.w);
     }
+    store_row<HALF>(a, rec.qrow, rec.head0 + h, D, d, out, top, sum);
+}
+
+constexpr size_t ring_bytes(int D) { return size_t(PA_WARPS) * (384 / D) * 2 * PA_TILE * D * 2; }
+
+// Opts the kernel into its largest shared memory, once a device.
+template <int D, bool HALF>
+cudaError_t allow_smem() {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done.load() >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(k_paged_attn<D, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             int(ring_bytes(D) + (PAGED_MAX_ROWS + 1) * sizeof(int)));
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+    return e;
+}
+
+template <int D, bool HALF>
+cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
+    const int group = a.heads / a.cache.kv_heads;
+    Split sp;
+    sp.per_kv = (group + PA_HEADS - 1) / PA_HEADS;
+    sp.pairs = a.cache.kv_heads * sp.per_kv;
+    const long long longest = a.window > 0 ? std::min(a.window, a.max_len) : a.max_len;
+    // short requests stay whole; units grow only where their number would pass 31 bits
+    long long unit = longest <= PA_WHOLE ? PA_WHOLE : PA_UNIT;
+    while (a.rows * ((longest + unit - 1) / unit) > INT_MAX) unit *= 2;
+    sp.unit = int(unit);
+    const long long units = (longest + unit - 1) / unit, most = a.rows * units * sp.pairs;
+    const int blocks = int(std::min(most, 2ll * sm_count()));
+    sp.join = units > 1;
+    sp.by_pair = (long long)a.rows * sp.pairs <= blocks;
+    const size_t smem = ring_bytes(D) + (a.rows + 1) * sizeof(int);
+    cudaError_t e = allow_smem<D, HALF>();
+    if (e == cudaSuccess) e = pdl_launch(k_paged_attn<D, HALF>, dim3(blocks), dim3(PA_THREADS), smem, s, a, sp);
+    if (e != cudaSuccess || !sp.join) return e;
+    const int records = sp.by_pair ? a.rows * sp.pairs : blocks;
+    return pdl_launch(k_paged_join<D, HALF>, dim3(records, std::min(group, PA_HEADS)), dim3(JOIN_THREADS), 0, s, a);
 }
 
 }  // namespace
 
-size_t paged_attention_workspace() { return 1 << 20; }
+size_t paged_attention_workspace() { return PA_WORKSPACE; }
 
 cudaError_t launch_paged_attention(const PagedAttnArgs& a, int head_dim, bool half, cudaStream_t s) {
-    const int group = a.heads / a.cache.kv_heads, per_kv = (group + PA_HEADS - 1) / PA_HEADS;
-    const dim3 grid(a.cache.kv_heads * per_kv, a.rows);
-    if (head_dim == 128) {
-        if (half) k_paged_attn<128, true><<<grid, PA_THREADS, 0, s>>>(a, group, per_kv);
-        else k_paged_attn<128, false><<<grid, PA_THREADS, 0, s>>>(a, group, per_kv);
-    } else {
-        if (half) k_paged_attn<64, true><<<grid, PA_THREADS, 0, s>>>(a, group, per_kv);
-        else k_paged_attn<64, false><<<grid, PA_THREADS, 0, s>>>(a, group, per_kv);
-    }
-    return cudaGetLastError();
+    if (head_dim == 128) return half ? launch<128, true>(a, s) : launch<128, false>(a, s);
+    return half ? launch<64, true>(a, s) : launch<64, false>(a, s);
 }
 
 }  // namespace plamo
