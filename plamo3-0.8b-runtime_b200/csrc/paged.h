@@ -2,6 +2,7 @@
 // paged_qkv.cu, paged_attn.cu and sample.cu. The public contract is in include/plamo_kernels.h; every
 // launcher expects arguments that paged_api.cu has checked.
 #pragma once
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -10,6 +11,17 @@ namespace plamo {
 
 constexpr int PAGED_MAX_ROWS = 8192;     // rows of a plan or an attention call: their prefix sums sit in shared memory
 constexpr int SAMPLE_MAX_VOCAB = 1 << 22;  // 2^22 weights of at most 2^40: sums below 2^62
+
+// Opts a kernel into `bytes` of dynamic shared memory, once a device (`done` remembers which).
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done.load() >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
+    return e;
+}
 
 struct PagedCacheArgs {
     uint16_t* keys;

@@ -22,7 +22,6 @@
 #include "paged.h"
 
 #include <algorithm>
-#include <atomic>
 #include <climits>
 
 namespace plamo {
@@ -492,19 +491,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a) {
 
 constexpr size_t ring_bytes(int D) { return size_t(PA_WARPS) * (384 / D) * 2 * PA_TILE * D * 2; }
 
-// Opts the kernel into its largest shared memory, once a device.
-template <int D, bool HALF>
-cudaError_t allow_smem() {
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 64 && (done.load() >> dev & 1))) return e;
-    e = cudaFuncSetAttribute(k_paged_attn<D, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             int(ring_bytes(D) + (PAGED_MAX_ROWS + 1) * sizeof(int)));
-    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev);
-    return e;
-}
-
 template <int D, bool HALF>
 cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
     const int group = a.heads / a.cache.kv_heads;
@@ -521,7 +507,8 @@ cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
     sp.join = units > 1;
     sp.by_pair = (long long)a.rows * sp.pairs <= blocks;
     const size_t smem = ring_bytes(D) + (a.rows + 1) * sizeof(int);
-    cudaError_t e = allow_smem<D, HALF>();
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_shared(k_paged_attn<D, HALF>, ring_bytes(D) + (PAGED_MAX_ROWS + 1) * sizeof(int), done);
     if (e == cudaSuccess) e = pdl_launch(k_paged_attn<D, HALF>, dim3(blocks), dim3(PA_THREADS), smem, s, a, sp);
     if (e != cudaSuccess || !sp.join) return e;
     const int records = sp.by_pair ? a.rows * sp.pairs : blocks;

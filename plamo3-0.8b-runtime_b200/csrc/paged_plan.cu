@@ -160,11 +160,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_paged_plan(PagedPlanArgs a) {
 
 cudaError_t launch_paged_plan(const PagedPlanArgs& a, cudaStream_t s) {
     const size_t smem = size_t(4) * a.rows * sizeof(int);
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(k_paged_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             4 * PAGED_MAX_ROWS * int(sizeof(int)));
-        if (e != cudaSuccess) return e;
-    }
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_shared(k_paged_plan, size_t(4) * PAGED_MAX_ROWS * sizeof(int), done);
+    if (e != cudaSuccess) return e;
     const long long work = (long long)a.tokens + 64ll * a.rows;
     const int blocks = int(std::clamp((work + 4 * PLAN_THREADS - 1) / (4 * PLAN_THREADS), 1ll, 148ll));
     k_paged_plan<<<blocks, PLAN_THREADS, smem, s>>>(a);
