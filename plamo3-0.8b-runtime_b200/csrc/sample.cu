@@ -9,12 +9,14 @@
 //
 // A cluster of up to 8 blocks takes a row: each keeps its slice of the logits in shared memory after one
 // read from global memory, and sums and histograms are exchanged through distributed shared memory, one
-// cluster barrier each. A threshold takes a histogram over 1024 equal steps of (max - x), which spreads
-// the many near-equal logits that bins by bits of x would pile onto a few addresses, then one over the
-// keys inside the chosen step (one for 16-bit logits, mostly two for fp32). What cannot be kept is skipped
-// before its exponential is taken: w = 0 beyond 27.8 T, and under top-p what V times over would not fill the
-// part that may be left out. Bound by instructions (an exponential an id at least) for many rows, by the
-// cluster barriers (3 to 9) for one.
+// cluster barrier each. A threshold takes a histogram over 512 equal steps of (max - x), which spreads
+// the many near-equal logits that bins by bits of x would pile onto a few addresses. When at most 1024 ids
+// lie up to the step where k or p is reached (nearly always: what is kept is a small head of the vocabulary)
+// they are sent to the first block, which sorts them and finishes the row alone. Else the threshold is
+// narrowed down by histograms over the keys inside the step, and all blocks finish the row.
+// What cannot be kept is skipped before its exponential is taken: w = 0 beyond 27.8 T, and under top-p what
+// V times over would not fill the part that may be left out. Bound by instructions (an exponential an id
+// at least, unless top-k comes first) for many rows, by the cluster barriers for one.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -31,7 +33,8 @@ namespace cg = cooperative_groups;
 
 constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
-constexpr int BINS = 1024;
+constexpr int BINS = SAMPLE_THREADS;     // one bin a thread
+constexpr int LIST = 1024;               // ids that the first block can finish alone
 constexpr int MAX_CLUSTER = 8;
 constexpr int SLICE_BYTES = 128 * 1024;  // most of a slice kept in shared memory; the rest is read again
 constexpr float SPAN = 27.8f;            // 2^40 exp(-27.8) < 1
@@ -73,10 +76,34 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(~(full | ((1u << SHIFT) - 1u)));
 }
 
-// x > -inf
-__device__ __forceinline__ u64 weight(float x, float top, float temperature) {
-    const float e = x == top ? 1.f : expf(__fdiv_rn(x - top, temperature));
-    return e > 0.f ? u64(e * 1099511627776.0f) : 0ull;
+// exp((x - top) / T) in fp32, 1 at the top; 0 or NaN where there is nothing to choose (-inf, NaN).
+// The quotient is the IEEE one (ids must not depend on how it is computed): with y = 1 / T rounded once, two
+// corrections q += (d - q T) y by fused multiply-adds round d / T correctly (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990), where nothing leaves the normal range.
+struct Likelihood {
+    float top, T, inv;
+    bool plain;  // T far from 1 or an infinite top: the compiler's division, and the top's own case
+    __device__ __forceinline__ void set(float top_, float T_) {
+        top = top_;
+        T = T_;
+        inv = __frcp_rn(T_);
+        plain = !(T_ > 1e-15f && T_ < 1e15f) || top_ == INFINITY;
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float d = x - top;
+        if (plain) return x == top && x > -INFINITY ? 1.f : expf(__fdiv_rn(d, T));
+        float q = d * inv;
+        q = fmaf(fmaf(-q, T, d), inv, q);
+        q = fmaf(fmaf(-q, T, d), inv, q);
+        return expf(q);
+    }
+};
+constexpr float LEAST = 9.094947017729282e-13f;  // 2^-40: anything less likely weighs nothing
+
+// floor(2^40 e), 2^-40 <= e <= 1
+__device__ __forceinline__ u64 fixed(float e) {
+    const uint32_t b = __float_as_uint(e);
+    return (u64((b & 0x7fffffu) | 0x800000u) << 17) >> (127u - (b >> 23));
 }
 
 // fraction * total / 2^24 in whole numbers (fraction <= 2^24, total < 2^62), rounded down or up
@@ -84,9 +111,25 @@ __device__ __forceinline__ u64 share(u64 fraction, u64 total, bool up) {
     return fraction * (total >> 24) + ((fraction * (total & 0xffffffull) + (up ? 0xffffffull : 0ull)) >> 24);
 }
 
+// ln(w / total) from whole numbers: near 1 by what is missing, so that no digits cancel
+__device__ __forceinline__ float log_share(u64 w, u64 total) {
+    if (2 * w > total) return log1pf(-__fdiv_rn(float(total - w), float(total)));
+    return logf(__fdiv_rn(float(w), float(total)));
+}
+
 __device__ __forceinline__ u64 warp_add(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+    return v;
+}
+
+// inclusive, in lane order
+__device__ __forceinline__ u64 warp_scan(u64 v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(FULL_MASK, v, o);
+        if ((threadIdx.x & 31) >= o) v += y;
+    }
     return v;
 }
 
@@ -96,11 +139,15 @@ struct Pair {
 
 struct Shared {
     u64 hist[2][BINS];  // two, used in turn: one may still be read by other blocks while the next fills
-    Pair exchange[4];   // likewise
+    uint32_t members[2][BINS];      // of a histogram of weights: how many values
+    Pair exchange[4][MAX_CLUSTER];  // likewise; [i][c] is written by block c
+    static_assert(LIST == 2 * SAMPLE_THREADS, "two entries a thread");
+    u64 list[LIST];     // the first block's: ~key << 32 | id, so ascending order is what ties need
+    uint32_t listed;
     Pair warp_pairs[SAMPLE_WARPS];
     u64 scan[SAMPLE_WARPS];
-    // a histogram's answer: the bin, the amount before it, the amount in it
-    u64 bin, before, amount;
+    // a histogram's answer: the bin, the amount before it, the amount in it, the values up to and in it
+    u64 bin, before, amount, upto;
 };
 
 template <int TYPE>
@@ -116,7 +163,8 @@ struct Row {
     int begin, length, cached;  // the block's values [begin, begin + length)
     int mine0, mine1;     // this thread's values, from begin
     int turn = 0, hist_turn = 0;
-    float top, temperature;
+    float top;
+    Likelihood like;
 
     __device__ Row(Shared& s) : sh(s) {}
 
@@ -126,7 +174,33 @@ struct Row {
         return id >= 0 && id < vocab ? row[id] : Logit<TYPE>::NOTHING;
     }
     __device__ __forceinline__ float at(int i) const { return Logit<TYPE>::value(raw_at(i)); }
+    // act(x, pure(x), i) for this thread's values in index order; four reads and four pure(x) are in flight
+    // together, so that their latencies overlap.
+    template <typename F, typename G>
+    __device__ __forceinline__ void each(F pure, G act) const {
+        constexpr int BATCH = 4;
+        int i = mine0;
+        for (const int end = min(mine1, cached); i + BATCH <= end; i += BATCH) {
+            float x[BATCH];
+            decltype(pure(0.f)) y[BATCH];
+#pragma unroll
+            for (int e = 0; e < BATCH; e++) x[e] = Logit<TYPE>::value(slice[i + e]);
+#pragma unroll
+            for (int e = 0; e < BATCH; e++) y[e] = pure(x[e]);
+#pragma unroll
+            for (int e = 0; e < BATCH; e++) act(x[e], y[e], i + e);
+        }
+        for (; i < mine1; i++) {
+            const float x = at(i);
+            act(x, pure(x), i);
+        }
+    }
     static __device__ __forceinline__ uint32_t key(float x) { return order_key(x) >> Logit<TYPE>::KEY_SHIFT; }
+
+    __device__ __forceinline__ u64 weight(float x) const {
+        const float e = like(x);
+        return e >= LEAST ? fixed(e) : 0ull;
+    }
 
     // Sums of both values over the block.
     __device__ __forceinline__ Pair block_add(Pair v) {
@@ -143,12 +217,12 @@ struct Row {
     // Every block's pair (already summed over the block) becomes known to all: their sum, and the sum over the
     // blocks before this one.
     __device__ __forceinline__ Pair exchange(Pair block, Pair& before) {
-        Pair* const place = &sh.exchange[turn++ & 3];
-        if (threadIdx.x == 0) *place = block;
+        Pair* const places = sh.exchange[turn++ & 3];
+        if (threadIdx.x < ranks) *cluster.map_shared_rank(places + rank, threadIdx.x) = block;
         cluster.sync();
         const int lane = threadIdx.x & 31;
         Pair p{0, 0};
-        if (lane < ranks) p = *cluster.map_shared_rank(place, lane);
+        if (lane < ranks) p = places[lane];
         before.a = warp_add(lane < rank ? p.a : 0ull);
         before.b = warp_add(lane < rank ? p.b : 0ull);
         return Pair{warp_add(p.a), warp_add(p.b)};
@@ -156,12 +230,7 @@ struct Row {
     // Exclusive running sum over the block in thread order.
     __device__ __forceinline__ u64 block_scan(u64 v) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        u64 x = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(FULL_MASK, x, o);
-            if (lane >= o) x += y;
-        }
+        const u64 x = warp_scan(v);
         __syncthreads();
         if (lane == 31) sh.scan[warp] = x;
         __syncthreads();
@@ -171,85 +240,185 @@ struct Row {
         return before + x - v;
     }
 
+    // The same for a team of threads: one warp or the block.
+    template <int TEAM>
+    __device__ __forceinline__ void team_sync() {
+        if (TEAM == 32) __syncwarp();
+        else __syncthreads();
+    }
+    template <int TEAM>
+    __device__ __forceinline__ Pair team_add(Pair v) {
+        if (TEAM == 32) return Pair{warp_add(v.a), warp_add(v.b)};
+        return block_add(v);
+    }
+    template <int TEAM>
+    __device__ __forceinline__ u64 team_scan(u64 v) {
+        if (TEAM == 32) return warp_scan(v) - v;
+        return block_scan(v);
+    }
+
     // One histogram over the cluster. classify(x) gives a value's bin (larger values in lower bins) or -1; an
     // entry counts 1, or its weight. Finds the first bin at which `base` and the amounts up to it reach `need`
-    // (left in sh.bin / before / amount); false when they do not.
+    // (left in sh.bin / before / amount / upto); false when they do not.
     template <bool WEIGHTS, typename F>
     __device__ __forceinline__ bool histogram(F classify, u64 base, u64 need) {
-        u64* const hist = sh.hist[hist_turn++ & 1];
-        uint32_t* const counts = reinterpret_cast<uint32_t*>(hist);
-        for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
-            if (WEIGHTS) hist[i] = 0;
-            else counts[i] = 0;
-        }
+        u64* const hist = sh.hist[hist_turn & 1];
+        uint32_t* const counts = sh.members[hist_turn++ & 1];
+        if (WEIGHTS) hist[threadIdx.x] = 0;
+        counts[threadIdx.x] = 0;
         if (threadIdx.x == 0) sh.bin = BINS;
         __syncthreads();
-        for (int i = mine0; i < mine1; i++) {
-            const float x = at(i);
-            const int bin = classify(x);
-            if (bin < 0) continue;
+        each(classify, [&](float x, int bin, int) {
+            if (bin < 0) return;
             if (WEIGHTS) {
-                const u64 w = weight(x, top, temperature);
-                if (w) atomicAdd(hist + bin, w);
-            } else {
-                atomicAdd(counts + bin, 1u);
+                const u64 w = weight(x);
+                if (!w) return;
+                atomicAdd(hist + bin, w);
             }
-        }
+            atomicAdd(counts + bin, 1u);
+        });
         cluster.sync();
-        constexpr int PER = BINS / SAMPLE_THREADS;
-        u64 sum[PER], all = 0;
+        u64 sum = 0, count = 0;
 #pragma unroll
-        for (int b = 0; b < PER; b++) sum[b] = 0;
-        for (int c = 0; c < ranks; c++) {
-            const u64* const h = cluster.map_shared_rank(hist, c);
-            const uint32_t* const n = reinterpret_cast<const uint32_t*>(h);
-#pragma unroll
-            for (int b = 0; b < PER; b++) sum[b] += WEIGHTS ? h[threadIdx.x * PER + b] : n[threadIdx.x * PER + b];
+        for (int c = 0; c < MAX_CLUSTER; c++) {  // all reads in flight together
+            if (c >= ranks) continue;
+            if (WEIGHTS) sum += cluster.map_shared_rank(hist, c)[threadIdx.x];
+            count += cluster.map_shared_rank(counts, c)[threadIdx.x];
         }
-#pragma unroll
-        for (int b = 0; b < PER; b++) all += sum[b];
-        u64 before = base + block_scan(all);
-#pragma unroll
-        for (int b = 0; b < PER; b++) {
-            if (before < need && need <= before + sum[b]) {
-                sh.bin = threadIdx.x * PER + b;
-                sh.before = before;
-                sh.amount = sum[b];
-            }
-            before += sum[b];
+        if (!WEIGHTS) sum = count;
+        const u64 before = base + block_scan(sum), counted = WEIGHTS ? block_scan(count) : before - base;
+        if (before < need && need <= before + sum) {
+            sh.bin = threadIdx.x;
+            sh.before = before;
+            sh.amount = sum;
+            sh.upto = counted + count;
         }
         __syncthreads();
         return sh.bin < BINS;
     }
 
-    // The key at which the amounts of the values, from the largest down, reach `need`; before and amount: the
-    // amounts above it and at it. Values more than `limit` below the largest do not matter. False when the
-    // amounts stay below `need`.
-    template <bool WEIGHTS>
-    __device__ __forceinline__ bool find(u64 need, float limit, uint32_t least_key, uint32_t& edge, u64& before, u64& amount) {
-        const float step = float(BINS) / limit;
-        auto coarse = [&](float x) -> int {
+    // Steps of (max - x) up to `limit` below the largest; -1 beyond it.
+    struct Steps {
+        float top, limit, step;
+        __device__ __forceinline__ int operator()(float x) const {
             const float d = top - x;
             if (!(x > -INFINITY) || d > limit) return -1;
             return min(int(d * step), BINS - 1);
-        };
-        auto within = [&](float x) -> int { return key(x) < least_key ? -1 : coarse(x); };
-        if (!histogram<WEIGHTS>(within, 0, need)) return false;
+        }
+    };
+
+    // Sends every value in a step up to `bin` to the first block's list; the number sent by the whole cluster.
+    __device__ __forceinline__ int gather(const Steps& steps, int bin, uint32_t least_key) {
+        uint32_t* const count = cluster.map_shared_rank(&sh.listed, 0);
+        u64* const list = cluster.map_shared_rank(sh.list, 0);
+        each([&](float x) { return key(x) < least_key ? -1 : steps(x); },
+             [&](float x, int b, int i) {
+                 if (b < 0 || b > bin) return;
+                 const uint32_t n = atomicAdd(count, 1u);
+                 if (n < LIST) list[n] = u64(~key(x)) << 32 | uint32_t(begin + i - lead);
+             });
+        cluster.sync();
+        return rank == 0 ? int(sh.listed) : 0;
+    }
+
+    // Sorts the list's first n entries ascending (n a power of two, at most 2 * TEAM): bitonic, in shared memory.
+    template <int TEAM>
+    __device__ __forceinline__ void sort_list(int n) {
+        for (int size = 2; size <= n; size *= 2)
+            for (int gap = size / 2; gap > 0; gap /= 2) {
+                team_sync<TEAM>();
+                if (threadIdx.x < n / 2) {
+                    const int i = threadIdx.x, lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
+                    const u64 a = sh.list[lo], b = sh.list[hi];
+                    if ((a > b) == ((lo & size) == 0)) {
+                        sh.list[lo] = b;
+                        sh.list[hi] = a;
+                    }
+                }
+            }
+        team_sync<TEAM>();
+    }
+
+    // The row's last steps, by the first TEAM threads of the first block (its first warp, or all): n ids on the
+    // list, n <= 2 * TEAM, hold everything that can be kept. run_known: the weight that top-p is a share of (0: that
+    // of the first k listed ones).
+    template <int TEAM>
+    __device__ __forceinline__ void finish_list(const SampleArgs& a, int r, int n, int k, u64 p24, u64 least, u64 m, u64 run_known) {
+        constexpr int KS = Logit<TYPE>::KEY_SHIFT;
+        const int t = threadIdx.x;
+        int size = 2;
+        while (size < n) size *= 2;
+        for (int i = n + t; i < size; i += TEAM) sh.list[i] = ~0ull;
+        sort_list<TEAM>(size);
+        u64 w[2];  // two neighbouring entries a thread
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int i = 2 * t + e;
+            w[e] = i < n && i < k ? weight(key_value<KS>(uint32_t(~sh.list[i] >> 32))) : 0ull;
+        }
+        const bool nucleus = p24 < (1ull << 24);
+        const u64 before = team_scan<TEAM>(w[0] + w[1]);
+        if (nucleus) {
+            const u64 run = run_known ? run_known : team_add<TEAM>({w[0] + w[1], 0}).a, need = max(share(p24, run, true), 1ull);
+            if (before + w[0] >= need) w[1] = 0;
+            if (before >= need) w[0] = 0;
+        }
+        if (w[0] < least) w[0] = 0;
+        if (w[1] < least) w[1] = 0;
+        const Pair total = team_add<TEAM>({w[0] + w[1], u64((w[0] != 0) + (w[1] != 0))});
+        // the kept ones are the first total.b; now in index order, each with its key
+        const int kept = int(total.b);
+        size = 2;
+        while (size < kept) size *= 2;
+        u64 entry[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) entry[e] = 2 * t + e < kept ? sh.list[2 * t + e] : 0ull;
+        team_sync<TEAM>();
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+            if (2 * t + e < size) sh.list[2 * t + e] = 2 * t + e < kept ? entry[e] << 32 | uint32_t(~entry[e] >> 32) : ~0ull;
+        sort_list<TEAM>(size);
+#pragma unroll
+        for (int e = 0; e < 2; e++) w[e] = 2 * t + e < kept ? weight(key_value<KS>(uint32_t(sh.list[2 * t + e]))) : 0ull;
+        const u64 target = share(m, total.a, false);
+        u64 upto = team_scan<TEAM>(w[0] + w[1]);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if (upto <= target && target < upto + w[e]) {
+                a.ids[r] = int(sh.list[2 * t + e] >> 32);
+                if (a.logprobs) a.logprobs[r] = log_share(w[e], total.a);
+            }
+            upto += w[e];
+        }
+        if (t == 0 && a.kept) a.kept[r] = kept;
+    }
+    __device__ __forceinline__ void finish_listed(const SampleArgs& a, int r, int n, int k, u64 p24, u64 least, u64 m, u64 run_known) {
+        if (rank != 0) return;
+        if (n > 64) finish_list<SAMPLE_THREADS>(a, r, n, k, p24, least, m, run_known);
+        else if (threadIdx.x < 32) finish_list<32>(a, r, n, k, p24, least, m, run_known);
+    }
+
+    // After histogram() over `steps`: the key at which the amounts of the values, from the largest down, reach
+    // `need`; before and amount: the amounts above it and at it.
+    template <bool WEIGHTS>
+    __device__ __forceinline__ void narrow(const Steps& steps, u64 need, uint32_t least_key, uint32_t& edge, u64& before,
+                                           u64& amount) {
         const int bin = int(sh.bin);
         u64 base = sh.before;
-        // keys that the bin can hold: its bounds, widened by more than the two roundings of `coarse`
-        const double low = bin == BINS - 1 ? double(limit) : (bin + 1) / double(step), high = bin ? bin / double(step) : 0.0;
+        // keys that the step can hold: its bounds, widened by more than the two roundings of `steps`
+        const double low = bin == BINS - 1 ? double(steps.limit) : (bin + 1) / double(steps.step),
+                     high = bin ? bin / double(steps.step) : 0.0;
         uint32_t khi = key(__double2float_ru(double(top) - high * (1.0 - 1e-6)));
         uint32_t klo = key(__double2float_rd(double(top) - low * (1.0 + 1e-6)));
         if (top == INFINITY) khi = klo = key(top);
         while (true) {
-            const int bits = 32 - __clz(khi - klo), shift = max(bits - 10, 0);
+            const int bits = 32 - __clz(khi - klo), shift = max(bits - 9, 0);
             __syncthreads();  // the answer before has been read
             auto fine = [&](float x) -> int {
                 const uint32_t k = key(x);
-                return k < least_key || k > khi || k < klo || coarse(x) != bin ? -1 : int((khi - k) >> shift);
+                return k < least_key || k > khi || k < klo || steps(x) != bin ? -1 : int((khi - k) >> shift);
             };
-            if (!histogram<WEIGHTS>(fine, base, need)) return false;  // cannot happen: the bin holds it
+            histogram<WEIGHTS>(fine, base, need);
             base = sh.before;
             khi -= uint32_t(sh.bin) << shift;
             if (!shift) break;
@@ -259,7 +428,6 @@ struct Row {
         before = base;
         amount = sh.amount;
         __syncthreads();
-        return true;
     }
 };
 
@@ -272,6 +440,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     Row<TYPE> row(shared);
     constexpr int VEC = Row<TYPE>::VEC;
     const int t = threadIdx.x, V = a.vocab;
+    row.cluster.barrier_arrive();  // waited for before the first access to another block's shared memory
     row.ranks = int(row.cluster.num_blocks());
     row.rank = int(row.cluster.block_rank());
     const int r = blockIdx.x / row.ranks;
@@ -295,60 +464,93 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     const float top_p = a.top_p ? a.top_p[r] : 1.f, min_p = a.min_p ? a.min_p[r] : 0.f, u = a.u[r];
     const u64 p24 = top_p < 1.f ? u64(rint(fmax(double(top_p), 0.0) * 16777216.0)) : 1ull << 24;
     const u64 least = max(1ull, min_p > 0.f ? u64(ceil(fmin(double(min_p), 1.0) * 1099511627776.0)) : 0ull);
-    row.temperature = T;
 
     // read the slice once; the largest logit (fmaxf passes over NaN)
     float top = -INFINITY;
-    for (int v = t; v * VEC < row.length; v += SAMPLE_THREADS) {
-        const int j = v * VEC, id = row.begin + j - row.lead;
-        raw x[VEC];
-        if (id >= 0 && id + VEC <= V) {
-            *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(row.row + id));
-        } else {
+    constexpr int BATCH = 4;  // reads in flight together
+    for (int v0 = t; v0 * VEC < row.length; v0 += BATCH * SAMPLE_THREADS) {
+        uint4 x4[BATCH];
 #pragma unroll
-            for (int e = 0; e < VEC; e++) x[e] = id + e >= 0 && id + e < V ? row.row[id + e] : Logit<TYPE>::NOTHING;
+        for (int b = 0; b < BATCH; b++) {
+            const int j = (v0 + b * SAMPLE_THREADS) * VEC, id = row.begin + j - row.lead;
+            if (j < row.length && id >= 0 && id + VEC <= V) {
+                x4[b] = __ldg(reinterpret_cast<const uint4*>(row.row + id));
+            } else {  // the row's ends
+                raw x[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    x[e] = j < row.length && id + e >= 0 && id + e < V ? row.row[id + e] : Logit<TYPE>::NOTHING;
+                x4[b] = *reinterpret_cast<const uint4*>(x);
+            }
         }
-        if (j < row.cached) *reinterpret_cast<uint4*>(row.slice + j) = *reinterpret_cast<const uint4*>(x);
 #pragma unroll
-        for (int e = 0; e < VEC; e++) top = fmaxf(top, Logit<TYPE>::value(x[e]));
+        for (int b = 0; b < BATCH; b++) {
+            const int j = (v0 + b * SAMPLE_THREADS) * VEC;
+            if (j < row.cached) *reinterpret_cast<uint4*>(row.slice + j) = x4[b];
+            const raw* x = reinterpret_cast<const raw*>(&x4[b]);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) top = fmaxf(top, Logit<TYPE>::value(x[e]));
+        }
     }
     top = warp_max(top);
     Pair unused;
     {
-        Pair* const place = &shared.exchange[row.turn++ & 3];
+        Pair* const places = shared.exchange[row.turn++ & 3];
         if ((t & 31) == 0) shared.scan[t >> 5] = __float_as_uint(top);
+        if (t == 0) shared.listed = 0;
         __syncthreads();
         top = warp_max(t % 32 < SAMPLE_WARPS ? __uint_as_float(uint32_t(shared.scan[t % 32])) : -INFINITY);
-        if (t == 0) place->a = __float_as_uint(top);
+        row.cluster.barrier_wait();
+        if (t < row.ranks) row.cluster.map_shared_rank(places + row.rank, t)->a = __float_as_uint(top);
         row.cluster.sync();
         const int lane = t & 31;
-        top = warp_max(lane < row.ranks ? __uint_as_float(uint32_t(row.cluster.map_shared_rank(place, lane)->a)) : -INFINITY);
+        top = warp_max(lane < row.ranks ? __uint_as_float(uint32_t(places[lane].a)) : -INFINITY);
     }
     row.top = top;
+    row.like.set(top, T);
+
+    const float far = SPAN * T;
+    const u64 m = u > 0.f ? min(u64(fminf(u, 1.f) * 16777216.0f), (1ull << 24) - 1) : 0ull;
+    const bool nucleus = p24 < (1ull << 24);
+    typedef typename Row<TYPE>::Steps Steps;
+    constexpr int KS = Logit<TYPE>::KEY_SHIFT;
 
     // kept: keys above `edge`, and the first `ties` (in index order) of the `at_edge` values at it
     uint32_t edge = 0;
     u64 ties = 0, at_edge = 0, before, amount;
-    if (k < V && row.template find<false>(k, SPAN * T, 0u, edge, before, amount)) {
-        at_edge = amount;
-        ties = k - before;
-    }
-    if (p24 < (1ull << 24)) {
-        Pair w{0, 0};
-        const float far = SPAN * T;
-        for (int i = row.mine0; i < row.mine1; i++) {
-            const float x = row.at(i);
-            if (x > -INFINITY && !(top - x > far) && row.key(x) >= edge) w.a += weight(x, top, T);
+    if (k < V) {
+        const Steps steps{top, far, float(BINS) / far};
+        if (row.template histogram<false>(steps, 0, k)) {
+            if (shared.upto <= LIST) {
+                row.finish_listed(a, r, row.gather(steps, int(shared.bin), 0u), k, p24, least, m, 0);
+                return;
+            }
+            row.template narrow<false>(steps, k, 0u, edge, before, amount);
+            at_edge = amount;
+            ties = k - before;
         }
-        const u64 one = ties < at_edge ? weight(key_value<Logit<TYPE>::KEY_SHIFT>(edge), top, T) : 0ull;
+    }
+    if (nucleus) {
+        Pair w{0, 0};
+        auto add = [&](float, float e, int) { w.a += e >= LEAST ? fixed(e) : 0ull; };
+        if (edge) row.each([&](float x) { return x > -INFINITY && row.key(x) >= edge ? row.like(x) : 0.f; }, add);
+        else row.each(row.like, add);
+        const u64 one = ties < at_edge ? row.weight(key_value<KS>(edge)) : 0ull;
         const u64 run = row.exchange(row.block_add(w), unused).a - (at_edge - ties) * one;
         const u64 need = max(share(p24, run, true), 1ull);
         // an id whose weight V times over fits into what may be left out is left out itself
         const u64 small = (run - min(need, run)) / u64(V);
         const float limit = small > 1 ? fminf(far, T * (log2f(1099511627776.0f / float(small)) * 0.6931472f) * 1.0001f + 1e-6f * T) : far;
-        uint32_t cut = edge;
-        if (run && row.template find<true>(need, limit, edge, cut, before, amount)) {
-            const u64 each = weight(key_value<Logit<TYPE>::KEY_SHIFT>(cut), top, T);
+        const Steps steps{top, limit, float(BINS) / limit};
+        auto within = [&](float x) -> int { return row.key(x) < edge ? -1 : steps(x); };
+        if (run && row.template histogram<true>(within, 0, need)) {
+            if (shared.upto <= LIST && ties == at_edge) {  // top-k has not cut through equal values
+                row.finish_listed(a, r, row.gather(steps, int(shared.bin), edge), k, p24, least, m, run);
+                return;
+            }
+            uint32_t cut = edge;
+            row.template narrow<true>(steps, need, edge, cut, before, amount);
+            const u64 each = row.weight(key_value<KS>(cut));
             ties = (need - before + each - 1) / each;
             at_edge = amount / each;
             edge = cut;
@@ -358,45 +560,60 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     u64 first_tie = 0;
     if (ties < at_edge) {
         u64 n = 0;
-        for (int i = row.mine0; i < row.mine1; i++) {
-            const float x = row.at(i);
-            n += x > -INFINITY && row.key(x) == edge;
-        }
+        row.each([&](float x) { return x > -INFINITY && row.key(x) == edge; }, [&](float, bool at, int) { n += at; });
         Pair ahead;
         row.exchange(row.block_add({n, 0}), ahead);
         first_tie = ahead.a + row.block_scan(n);
     }
-    const float far = SPAN * T;
-    auto kept_weight = [&](int i, u64& tie) -> u64 {
-        const float x = row.at(i);
-        if (!(x > -INFINITY) || top - x > far) return 0ull;
-        const uint32_t key = row.key(x);
-        if (key < edge || (key == edge && ties < at_edge && tie++ >= ties)) return 0ull;
-        const u64 w = weight(x, top, T);
-        return w >= least ? w : 0ull;
+    // w >= least, both whole, is e >= least / 2^40: exact in fp32, min_p having 24 bits
+    const float least_e = float(least) * LEAST;
+    const uint32_t tie_end = ties < at_edge ? uint32_t(ties) : 0xffffffffu;
+    u64 my_weight = 0;
+    uint32_t my_count = 0, tie = uint32_t(first_tie);
+    auto add = [&](float e) {
+        if (e >= least_e) {
+            my_weight += fixed(e);
+            my_count++;
+        }
     };
-    Pair mine{0, 0};
-    u64 tie = first_tie;
-    for (int i = row.mine0; i < row.mine1; i++) {
-        const u64 w = kept_weight(i, tie);
-        mine.a += w;
-        mine.b += w != 0;
+    if (edge) {
+        row.each([&](float x) { return x > -INFINITY ? row.key(x) : 0u; },
+                 [&](float x, uint32_t key, int) {
+                     if (key > edge || (key == edge && tie++ < tie_end)) add(row.like(x));
+                 });
+    } else {
+        row.each(row.like, [&](float, float e, int) { add(e); });
     }
     Pair ahead;
-    const Pair total = row.exchange(row.block_add(mine), ahead);
-    const u64 m = u > 0.f ? min(u64(fminf(u, 1.f) * 16777216.0f), (1ull << 24) - 1) : 0ull;
+    const Pair total = row.exchange(row.block_add({my_weight, my_count}), ahead);
     const u64 target = share(m, total.a, false);
-    u64 upto = ahead.a + row.block_scan(mine.a);
-    if (upto <= target && target < upto + mine.a) {
-        tie = first_tie;
-        for (int i = row.mine0; i < row.mine1; i++) {
-            const u64 w = kept_weight(i, tie);
-            if (target < upto + w) {
-                a.ids[r] = row.begin + i - row.lead;
-                if (a.logprobs) a.logprobs[r] = float(log(double(w) / double(total.a)));
+    const u64 upto = ahead.a + row.block_scan(my_weight);
+    // the thread whose values hold the target: its warp looks through them, a value a lane
+    const unsigned holds = __ballot_sync(FULL_MASK, upto <= target && target < upto + my_weight);
+    if (holds) {
+        const int owner = __ffs(holds) - 1, lane = t & 31;
+        const int i1 = __shfl_sync(FULL_MASK, row.mine1, owner);
+        u64 run = __shfl_sync(FULL_MASK, upto, owner);
+        uint32_t seen = __shfl_sync(FULL_MASK, uint32_t(first_tie), owner);
+        for (int i0 = __shfl_sync(FULL_MASK, row.mine0, owner); i0 < i1; i0 += 32) {
+            const int i = i0 + lane;
+            const float x = i < i1 ? row.at(i) : -INFINITY;
+            const uint32_t key = row.key(x);
+            const unsigned equal = __ballot_sync(FULL_MASK, x > -INFINITY && edge && key == edge);
+            const bool in = x > -INFINITY && (key > edge || !edge || (key == edge && seen + __popc(equal & ((1u << lane) - 1u)) < tie_end));
+            seen += __popc(equal);
+            const float e = row.like(x);
+            const u64 w = in && e >= least_e ? fixed(e) : 0ull;
+            const u64 incl = warp_scan(w);
+            const unsigned past = __ballot_sync(FULL_MASK, target < run + incl);
+            if (past) {
+                if (lane == __ffs(past) - 1) {
+                    a.ids[r] = row.begin + i - row.lead;
+                    if (a.logprobs) a.logprobs[r] = log_share(w, total.a);
+                }
                 break;
             }
-            upto += w;
+            run += __shfl_sync(FULL_MASK, incl, 31);
         }
     }
     if (row.rank == 0 && t == 0) {
@@ -406,15 +623,15 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
             if (a.logprobs) a.logprobs[r] = -INFINITY;
         }
     }
-    row.cluster.sync();  // no block leaves while another may read its shared memory
+    // no block reads another's shared memory after the last exchange, so each may leave by itself
 }
 
 template <int TYPE>
 cudaError_t launch(const SampleArgs& a, cudaStream_t s) {
     constexpr int SIZE = TYPE == 2 ? 4 : 2, VEC = 16 / SIZE;
-    // blocks a row: enough to keep slices in shared memory, more while the rows leave SMs idle
+    // blocks a row: enough that two blocks' slices fit an SM, more while all blocks still run at once
     int ranks = 1;
-    while (ranks < MAX_CLUSTER && ((long long)a.vocab * SIZE > (long long)ranks * SLICE_BYTES / 2 || a.rows * ranks < 296) &&
+    while (ranks < MAX_CLUSTER && ((long long)a.vocab * SIZE > (long long)ranks * (SLICE_BYTES / 4 * 3) || a.rows * ranks <= 148) &&
            a.vocab / ranks > 2048)
         ranks *= 2;
     const int len = ((a.vocab + VEC - 1 + ranks - 1) / ranks + VEC - 1) / VEC * VEC;
