@@ -4,8 +4,9 @@
 // in one pass over the keys with a running maximum and sum. Scores are kept in powers of two.
 //
 // Split. The work is a line of units (64 keys of one request and one KV head, at most 16 of its query
-// heads: the rows of an m16n8k16 MMA), request after request. Each block takes one stretch of equal length
-// of that line, whatever the lengths are, so a batch of any raggedness ends in one wave. The lengths are
+// heads: the rows of an m16n8k16 MMA), request after request, with a few empty places before each request
+// and head for what beginning it costs. Each block takes one stretch of equal length of that line,
+// whatever the lengths are, so a batch of any raggedness ends in one wave. The lengths are
 // on the device: every block adds them up itself. A request and head inside one stretch is finished there;
 // one that is cut leaves an fp32 partial per block, and k_paged_join adds those up in order, so a
 // result does not depend on timing. Calls whose requests cannot be cut launch no join.
@@ -23,6 +24,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace plamo {
 namespace {
@@ -34,8 +36,10 @@ constexpr int PA_TILE = 16;   // keys of a tile
 constexpr int PA_UNIT = 64;   // keys of a unit: one tile for each warp
 // Requests of at most this many keys are one unit and never cut.
 constexpr int PA_WHOLE = 256;
+// What beginning a request and head costs a block, in units: its share of the line is that much longer.
+constexpr int PA_BEGIN = 3;
 constexpr int PA_MAX_BLOCKS = 592;
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 512;
 // tiles in a warp's ring: 96 KB a block, two blocks an SM
 template <int D>
 constexpr int PA_STAGES = 384 / D;
@@ -197,24 +201,16 @@ int sm_count() {
     return n;
 }
 
-// What k_paged_join needs of one cut request and head: its query row (-1: nothing to join), heads, the blocks
-// first_block ... first_block + pieces - 1 that hold a piece, and the first one's place.
-struct __align__(16) JoinRecord {
-    int qrow, head0, heads, pieces;
-    int first_slot, first_block, pad0, pad1;
-};
-// Workspace: records, then 2 partials a block (the stretch's first and its last request), each 16 heads x
-// head_dim outputs, then 2 x 16 (maximum, sum) pairs a block.
-constexpr size_t PA_PART_AT = size_t(PA_MAX_BLOCKS) * sizeof(JoinRecord);
-constexpr size_t PA_STATS_AT = PA_PART_AT + size_t(2) * PA_MAX_BLOCKS * PA_HEADS * 128 * sizeof(float);
+// Workspace: 2 partials a block (of the first and the last request of its stretch), each 16 heads x head_dim
+// outputs, then 2 x 16 (maximum, sum) pairs a block.
+constexpr size_t PA_STATS_AT = size_t(2) * PA_MAX_BLOCKS * PA_HEADS * 128 * sizeof(float);
 constexpr size_t PA_WORKSPACE = PA_STATS_AT + size_t(2) * PA_MAX_BLOCKS * PA_HEADS * sizeof(float2);
 
 struct Split {
     int unit;       // keys of a unit
     int pairs;      // (KV head, block of 16 query heads) pairs of a request
     int per_kv;     // blocks of 16 query heads of a KV head
-    int by_pair;    // join records are indexed by (request, pair), else by block
-    int join;       // a join follows
+    int blocks;     // of k_paged_attn
 };
 
 // The query row of request r, -1 when it has none.
@@ -227,6 +223,72 @@ __device__ __forceinline__ int query_row(const PagedAttnArgs& a, int r) {
     return q >= 0 && q < a.q_rows ? q : -1;
 }
 
+// The line of work: upto[r] places lie before request r.
+struct Line {
+    const int* upto;
+    int total, per_block;
+    // A request and head, and where on the line they are.
+    struct Place {
+        int r, pair, begin, length;
+    };
+    __device__ __forceinline__ int begin_of(int block) const { return int(min((long long)block * per_block, (long long)total)); }
+    __device__ __forceinline__ Place at(int x, int rows, int pairs) const {
+        // the last request that begins at or before x
+        const int line = x / pairs;  // upto[mid] * pairs <= x
+        int lo = 0, hi = rows - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (upto[mid] <= line) lo = mid;
+            else hi = mid - 1;
+        }
+        Place p;
+        p.r = lo;
+        p.length = upto[lo + 1] - upto[lo];
+        const int inside = x - upto[lo] * pairs;
+        p.pair = inside / p.length;
+        p.begin = x - (inside - p.pair * p.length);
+        return p;
+    }
+};
+
+// Every block adds up the requests' places itself: the lengths are on the device, and this costs one read of
+// them. `upto` is shared memory for rows + 1 sums.
+template <int THREADS>
+__device__ __forceinline__ Line lay_out(const PagedAttnArgs& a, const Split& sp, int* upto) {
+    __shared__ int warp_sums[THREADS / 32];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const int per = (a.rows + THREADS - 1) / THREADS, r0 = min(t * per, a.rows), r1 = min(r0 + per, a.rows);
+    int sum = 0;
+    for (int r = r0; r < r1; r++) {
+        const int n = min(max(a.lens[r], 0), a.max_len), seen = a.window > 0 ? min(n, a.window) : n;
+        const int units = query_row(a, r) >= 0 ? (seen + sp.unit - 1) / sp.unit : 0;
+        const int places = units ? units + PA_BEGIN : 0;
+        upto[r + 1] = places;
+        sum += places;
+    }
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(FULL_MASK, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int at = x - sum;
+    for (int w = 0; w < warp; w++) at += warp_sums[w];
+    for (int r = r0; r < r1; r++) {
+        at += upto[r + 1];
+        upto[r + 1] = at;
+    }
+    if (t == 0) upto[0] = 0;
+    __syncthreads();
+    Line line;
+    line.upto = upto;
+    line.total = upto[a.rows] * sp.pairs;  // below 2^31 by the choice of the unit
+    line.per_block = max(1, int((unsigned(line.total) + sp.blocks - 1u) / unsigned(sp.blocks)));
+    return line;
+}
+
 template <int D, bool HALF>
 __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, Split sp) {
     pdl_enter();
@@ -234,106 +296,42 @@ __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, S
     extern __shared__ __align__(128) uint8_t pa_smem[];
     // the warps' rings, afterwards the warps' outputs; then the running sums of the requests' units
     constexpr int RING_BYTES = PA_WARPS * S * 2 * TILE_BYTES;
-    static_assert(PA_WARPS * PA_HEADS * D * 4 <= RING_BYTES, "the outputs fit in the rings");
+    constexpr int PITCH = D + 8;  // a warp's outputs, a head a row: 8 floats further than a multiple of 32 banks
+    static_assert(PA_WARPS * PA_HEADS * PITCH * 4 <= RING_BYTES, "the outputs fit in the rings");
     int* const upto = reinterpret_cast<int*>(pa_smem + RING_BYTES);  // [rows + 1]
     __shared__ float2 stats[PA_WARPS][PA_HEADS];
-    __shared__ int warp_sums[PA_WARPS];
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gq = lane >> 2, tq = lane & 3;
-    JoinRecord* const records = static_cast<JoinRecord*>(a.workspace);
-    float* const parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + PA_PART_AT);
+    float* const parts = static_cast<float*>(a.workspace);
     float2* const part_stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.workspace) + PA_STATS_AT);
-
-    // running sums of the units
-    {
-        const int per = (a.rows + PA_THREADS - 1) / PA_THREADS, r0 = min(t * per, a.rows), r1 = min(r0 + per, a.rows);
-        int sum = 0;
-        for (int r = r0; r < r1; r++) {
-            const int n = min(max(a.lens[r], 0), a.max_len), seen = a.window > 0 ? min(n, a.window) : n;
-            const int units = query_row(a, r) >= 0 ? (seen + sp.unit - 1) / sp.unit : 0;
-            upto[r + 1] = units;
-            sum += units;
-        }
-        int x = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(FULL_MASK, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) warp_sums[warp] = x;
-        __syncthreads();
-        int at = x - sum;
-        for (int w = 0; w < warp; w++) at += warp_sums[w];
-        for (int r = r0; r < r1; r++) {
-            at += upto[r + 1];
-            upto[r + 1] = at;
-        }
-        if (t == 0) upto[0] = 0;
-        __syncthreads();
-    }
-    const long long total = (long long)upto[a.rows] * sp.pairs;
-    const long long per_block = max((total + gridDim.x - 1) / gridDim.x, 1ll);
-    const long long x0 = min(blockIdx.x * per_block, total), x1 = min(x0 + per_block, total);
+    const Line line = lay_out<PA_THREADS>(a, sp, upto);
+    const int x0 = line.begin_of(blockIdx.x), x1 = line.begin_of(blockIdx.x + 1);
 
     // requests that see nothing
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         if (upto[r + 1] != upto[r]) continue;
-        if (sp.join && sp.by_pair)
-            for (int p = t; p < sp.pairs; p += PA_THREADS) records[r * sp.pairs + p].qrow = -1;
         const int qrow = query_row(a, r);
         if (qrow < 0) continue;
         for (int i = t; i < a.heads * D; i += PA_THREADS) a.out[qrow * a.out_stride + i] = 0;
         if (a.lse)
             for (int h = t; h < a.heads; h += PA_THREADS) a.lse[size_t(qrow) * a.heads + h] = -INFINITY;
     }
-    if (sp.join && !sp.by_pair && t == 0) {
-        // record of this block: the request and head that reach into its stretch from the block before,
-        // when no earlier block begins inside them (written below once they are known)
-        if (x0 >= x1) records[blockIdx.x].qrow = -1;
-    }
 
     const int group = a.heads / a.cache.kv_heads;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(pa_smem)) + warp * S * 2 * TILE_BYTES;
-    for (long long x = x0; x < x1;) {
-        // the request of unit x: the last one whose units begin at or before it
-        int lo = 0, hi = a.rows - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if ((long long)upto[mid] * sp.pairs <= x) lo = mid;
-            else hi = mid - 1;
-        }
-        const int r = lo, units = upto[r + 1] - upto[r];
-        const long long inside = x - (long long)upto[r] * sp.pairs;
-        const int pair = int(inside / units), u = int(inside - (long long)pair * units);
-        const int take = int(min((long long)(units - u), x1 - x));
-        const int kv = pair / sp.per_kv, h0 = (pair % sp.per_kv) * PA_HEADS;
+    for (int x = x0; x < x1;) {
+        const Line::Place at = line.at(x, a.rows, sp.pairs);
+        const int r = at.r, units = at.length - PA_BEGIN, place = x - at.begin;
+        const int stop = min(at.length, place + (x1 - x));
+        const int u = max(place - PA_BEGIN, 0), take = stop - PA_BEGIN - u;  // its units here: [u, u + take)
+        const int slot = 2 * blockIdx.x + (x != x0);
+        x += stop - place;
+        if (take <= 0) continue;
+        const int kv = at.pair / sp.per_kv, h0 = (at.pair % sp.per_kv) * PA_HEADS;
         const int heads = min(PA_HEADS, group - h0), head0 = kv * group + h0;
         const int qrow = query_row(a, r);
         const int n = min(max(a.lens[r], 0), a.max_len), first = a.window > 0 ? max(0, n - a.window) : 0;
         const int k0 = first + u * sp.unit, k1 = min((long long)n, k0 + (long long)take * sp.unit);
         const bool whole = take == units;
-        if (sp.join && t == 0) {
-            const long long begin = x - u;  // the pair's first unit on the line
-            const int b0 = int(begin / per_block), b1 = int((begin + units - 1) / per_block);
-            const JoinRecord rec{b1 > b0 ? qrow : -1, head0, heads, b1 - b0 + 1, 2 * b0 + (begin != b0 * per_block), b0, 0, 0};
-            if (sp.by_pair) {
-                if (u == 0) records[r * sp.pairs + pair] = rec;
-            } else if (x == x0) {
-                records[blockIdx.x] = rec;
-                if (u == 0 || (int)blockIdx.x != b0 + 1) records[blockIdx.x].qrow = -1;
-            }
-        }
-        // queries: rows gq and gq + 8 of the MMA
-        uint32_t qa[D / 16][4];
-        const uint16_t* q = a.q + qrow * a.q_stride + head0 * D;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int h = gq + (i & 1) * 8, d = kk * 16 + 2 * tq + (i >> 1) * 8;
-                qa[kk][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + h * D + d) : 0u;
-            }
-        Running<D> run;
-        run.clear();
         const int* table = a.table + size_t(r) * a.table_stride;
         const int tiles = (k1 - k0 + PA_TILE - 1) / PA_TILE;
         const int mine = tiles > warp ? (tiles - warp + PA_WARPS - 1) / PA_WARPS : 0;
@@ -359,27 +357,41 @@ __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, S
             }
             return mask;
         };
-        uint32_t masks[S];  // of the tiles in flight, oldest first
-        int next = page_of(0);
+        int pages[S];  // the lookups of the next tiles to copy, the ring's first ones together
 #pragma unroll
-        for (int s = 0; s < S - 1; s++) {
-            const int page = next;
-            next = page_of(s + 1);
-            masks[s] = s < mine ? issue(s, page) : 0u;
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-        for (int j = 0; j < mine; j++) {
-            const int page = next;
-            next = page_of(j + S);
-            masks[S - 1] = j + S - 1 < mine ? issue(j + S - 1, page) : 0u;
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-            __syncwarp();
-            const uint32_t kt = ring + (j % S) * 2 * TILE_BYTES;
-            add_tile<D, HALF>(run, qa, kt, kt + TILE_BYTES, masks[0], a.scale_log2);
-            __syncwarp();  // the tile has been read: the next copy may overwrite it
+        for (int i = 0; i < S; i++) pages[i] = page_of(i);
+        // queries: rows gq and gq + 8 of the MMA
+        uint32_t qa[D / 16][4];
+        const uint16_t* q = a.q + qrow * a.q_stride + head0 * D;
 #pragma unroll
-            for (int s = 0; s < S - 1; s++) masks[s] = masks[s + 1];
+        for (int kk = 0; kk < D / 16; kk++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int h = gq + (i & 1) * 8, d = kk * 16 + 2 * tq + (i >> 1) * 8;
+                qa[kk][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + h * D + d) : 0u;
+            }
+        Running<D> run;
+        run.clear();
+        // tile j is copied while tile j - (S - 1) is worked on
+        uint32_t masks[S];
+#pragma unroll
+        for (int i = 0; i < S; i++) masks[i] = 0u;
+#pragma unroll 1
+        for (int j = 0; j < mine + S - 1; j++) {
+            masks[S - 1] = j < mine ? issue(j, pages[0]) : 0u;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < S - 1; i++) pages[i] = pages[i + 1];
+            pages[S - 1] = page_of(j + S);
+            if (j >= S - 1) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+                __syncwarp();
+                const uint32_t kt = ring + ((j + 1) % S) * 2 * TILE_BYTES;
+                add_tile<D, HALF>(run, qa, kt, kt + TILE_BYTES, masks[0], a.scale_log2);
+                __syncwarp();  // the tile has been read: the next copy may overwrite it
+            }
+#pragma unroll
+            for (int i = 0; i < S - 1; i++) masks[i] = masks[i + 1];
         }
         // join the warps
 #pragma unroll
@@ -391,29 +403,34 @@ __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, S
         __syncthreads();  // every warp is done with its ring
         float* const mid = reinterpret_cast<float*>(pa_smem);
 #pragma unroll
-        for (int j = 0; j < D / 8; j++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                *reinterpret_cast<float2*>(mid + (warp * PA_HEADS + gq + 8 * h) * D + j * 8 + 2 * tq) =
-                    make_float2(run.o[j][2 * h], run.o[j][2 * h + 1]);
-        __syncthreads();
-        const int slot = 2 * blockIdx.x + (x != x0);
-        for (int i = t; i < heads * (D / 4); i += PA_THREADS) {
-            const int h = i / (D / 4), d = (i % (D / 4)) * 4;
+        for (int h = 0; h < 2; h++) {
             float m = -INFINITY;
 #pragma unroll
+            for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][gq + 8 * h].x);
+            const float f = ex2(run.m[h] - origin(m));
+#pragma unroll
+            for (int j = 0; j < D / 8; j++)
+                *reinterpret_cast<float2*>(mid + (warp * PA_HEADS + gq + 8 * h) * PITCH + j * 8 + 2 * tq) =
+                    make_float2(run.o[j][2 * h] * f, run.o[j][2 * h + 1] * f);
+        }
+        __syncthreads();
+        constexpr int ITEMS = PA_HEADS * D / 4 / PA_THREADS;
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            const int item = i * PA_THREADS + t, h = item / (D / 4), d = (item % (D / 4)) * 4;
+            if (h >= heads) break;
+            float m = -INFINITY, l = 0.f;
+#pragma unroll
             for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][h].x);
-            float l = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < PA_WARPS; w++) {
-                const float f = ex2(stats[w][h].x - origin(m));
-                const float4 v = *reinterpret_cast<const float4*>(mid + (w * PA_HEADS + h) * D + d);
-                l = fmaf(stats[w][h].y, f, l);
-                o.x = fmaf(v.x, f, o.x);
-                o.y = fmaf(v.y, f, o.y);
-                o.z = fmaf(v.z, f, o.z);
-                o.w = fmaf(v.w, f, o.w);
+                const float4 v = *reinterpret_cast<const float4*>(mid + (w * PA_HEADS + h) * PITCH + d);
+                l = fmaf(stats[w][h].y, ex2(stats[w][h].x - origin(m)), l);
+                o.x += v.x;
+                o.y += v.y;
+                o.z += v.z;
+                o.w += v.w;
             }
             if (whole) {
                 store_row<HALF>(a, qrow, head0 + h, D, d, o, m, l);
@@ -423,40 +440,69 @@ __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, S
             }
         }
         __syncthreads();  // the rings and stats are free again
-        x += take;
     }
 }
 
-// Adds up the pieces of one head of a cut request: warp w takes every eighth piece, then the warps are added.
+// Adds up the pieces of the heads of a cut request. A block takes 16 / per_head heads, per_head warps each: a
+// warp adds every per_head-th piece, then the warps of a head are added. Block x finds its request and head
+// on the line before it waits for the pieces: request and head x, or, when there are more of those than
+// blocks, the one that block x of k_paged_attn begins inside.
 template <int D, bool HALF>
-__global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a) {
-    pdl_enter();
+__global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Split sp, int by_pair, int per_head) {
     constexpr int WARPS = JOIN_THREADS / 32, VEC = D / 32;
-    __shared__ float outs[WARPS][D];
+    typedef typename std::conditional<D == 128, float4, float2>::type Vec;
+    extern __shared__ int join_upto[];  // [rows + 1]
+    __shared__ __align__(16) float outs[WARPS][D];
     __shared__ float2 stats[WARPS];
-    const JoinRecord rec = static_cast<const JoinRecord*>(a.workspace)[blockIdx.x];
-    const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (rec.qrow < 0 || h >= rec.heads) return;
-    const float* const parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + PA_PART_AT);
+    // The lengths may be read here: whatever wrote them ended before k_paged_attn began.
+    const Line line = lay_out<JOIN_THREADS>(a, sp, join_upto);
+    Line::Place at;
+    bool mine;
+    if (by_pair) {
+        at.r = blockIdx.x / sp.pairs;
+        at.pair = blockIdx.x % sp.pairs;
+        at.length = join_upto[at.r + 1] - join_upto[at.r];
+        at.begin = join_upto[at.r] * sp.pairs + at.pair * at.length;
+        mine = at.length > 0;
+    } else {
+        const int x = line.begin_of(blockIdx.x);
+        mine = x < line.total;
+        if (mine) at = line.at(x, a.rows, sp.pairs);
+    }
+    int b0 = 0, pieces = 0;  // the blocks that hold a piece: b0 ... b0 + pieces - 1
+    if (mine) {
+        b0 = (at.begin + PA_BEGIN) / line.per_block;
+        pieces = (at.begin + at.length - 1) / line.per_block - b0 + 1;
+        mine = pieces > 1 && (by_pair || int(blockIdx.x) == b0 + 1);
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.cache.kv_heads;
+    const int kv = mine ? at.pair / sp.per_kv : 0, h0 = mine ? (at.pair % sp.per_kv) * PA_HEADS : 0;
+    const int h = blockIdx.y * (WARPS / per_head) + warp / per_head, part = warp % per_head;
+    const int first_slot = 2 * b0 + (mine && at.begin > b0 * line.per_block);
+    pdl_enter();
+    if (!mine) return;
+    const int qrow = query_row(a, at.r);
+    const float* const parts = static_cast<const float*>(a.workspace);
     const float2* const part_stats = reinterpret_cast<const float2*>(static_cast<const uint8_t*>(a.workspace) + PA_STATS_AT);
-    float m = -INFINITY, l = 0.f, o[VEC];
+    float m = -INFINITY, l = 0.f;
+    __align__(16) float o[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) o[i] = 0.f;
-    constexpr int BATCH = 4;  // pieces whose reads are in flight together
-    for (int p0 = warp; p0 < rec.pieces; p0 += WARPS * BATCH) {
+    constexpr int BATCH = 6;  // pieces whose reads are in flight together
+    const bool inside = h < min(PA_HEADS, group - h0);
+    for (int p0 = inside ? part : pieces; p0 < pieces; p0 += per_head * BATCH) {
         float2 st[BATCH];
-        float v[BATCH][VEC];
+        __align__(16) float v[BATCH][VEC];
 #pragma unroll
         for (int b = 0; b < BATCH; b++) {
-            const int p = p0 + b * WARPS, slot = p == 0 ? rec.first_slot : 2 * (rec.first_block + p);
+            const int p = p0 + b * per_head, slot = p == 0 ? first_slot : 2 * (b0 + p);
             st[b] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int i = 0; i < VEC; i++) v[b][i] = 0.f;
-            if (p < rec.pieces) {
+            if (p < pieces) {
                 st[b] = part_stats[slot * PA_HEADS + h];
-                const float* src = parts + (size_t(slot) * PA_HEADS + h) * D + lane * VEC;
-#pragma unroll
-                for (int i = 0; i < VEC; i++) v[b][i] = src[i];
+                *reinterpret_cast<Vec*>(v[b]) =
+                    *reinterpret_cast<const Vec*>(parts + (size_t(slot) * PA_HEADS + h) * D + lane * VEC);
             }
         }
 #pragma unroll
@@ -468,16 +514,15 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a) {
             m = top;
         }
     }
-#pragma unroll
-    for (int i = 0; i < VEC; i++) outs[warp][lane * VEC + i] = o[i];
+    *reinterpret_cast<Vec*>(&outs[warp][lane * VEC]) = *reinterpret_cast<const Vec*>(o);
     if (lane == 0) stats[warp] = make_float2(m, l);
     __syncthreads();
-    if (threadIdx.x >= D / 4) return;
-    const int d = threadIdx.x * 4;
+    if (part != 0 || !inside || lane * 4 >= D) return;
+    const int d = lane * 4;
     float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < WARPS; w++) top = fmaxf(top, stats[w].x);
+    for (int w = warp; w < warp + per_head; w++) top = fmaxf(top, stats[w].x);
     float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < WARPS; w++) {
+    for (int w = warp; w < warp + per_head; w++) {
         const float f = ex2(stats[w].x - origin(top));
         const float4 v = *reinterpret_cast<const float4*>(&outs[w][d]);
         sum = fmaf(stats[w].y, f, sum);
@@ -486,7 +531,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a) {
         out.z = fmaf(v.z, f, out.z);
         out.w = fmaf(v.w, f, out.w);
     }
-    store_row<HALF>(a, rec.qrow, rec.head0 + h, D, d, out, top, sum);
+    store_row<HALF>(a, qrow, kv * group + h0 + h, D, d, out, top, sum);
 }
 
 constexpr size_t ring_bytes(int D) { return size_t(PA_WARPS) * (384 / D) * 2 * PA_TILE * D * 2; }
@@ -500,19 +545,24 @@ cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
     const long long longest = a.window > 0 ? std::min(a.window, a.max_len) : a.max_len;
     // short requests stay whole; units grow only where their number would pass 31 bits
     long long unit = longest <= PA_WHOLE ? PA_WHOLE : PA_UNIT;
-    while (a.rows * ((longest + unit - 1) / unit) > INT_MAX) unit *= 2;
+    while (a.rows * ((longest + unit - 1) / unit + PA_BEGIN) * sp.pairs > INT_MAX / 2) unit *= 2;
     sp.unit = int(unit);
-    const long long units = (longest + unit - 1) / unit, most = a.rows * units * sp.pairs;
-    const int blocks = int(std::min(most, 2ll * sm_count()));
-    sp.join = units > 1;
-    sp.by_pair = (long long)a.rows * sp.pairs <= blocks;
-    const size_t smem = ring_bytes(D) + (a.rows + 1) * sizeof(int);
+    const long long units = (longest + unit - 1) / unit;
+    sp.blocks = int(std::min(a.rows * sp.pairs * (units > 1 ? units + PA_BEGIN : 1), 2ll * sm_count()));
+    const size_t sums = (a.rows + 1) * sizeof(int), smem = ring_bytes(D) + sums;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_shared(k_paged_attn<D, HALF>, ring_bytes(D) + (PAGED_MAX_ROWS + 1) * sizeof(int), done);
-    if (e == cudaSuccess) e = pdl_launch(k_paged_attn<D, HALF>, dim3(blocks), dim3(PA_THREADS), smem, s, a, sp);
-    if (e != cudaSuccess || !sp.join) return e;
-    const int records = sp.by_pair ? a.rows * sp.pairs : blocks;
-    return pdl_launch(k_paged_join<D, HALF>, dim3(records, std::min(group, PA_HEADS)), dim3(JOIN_THREADS), 0, s, a);
+    if (e == cudaSuccess) e = pdl_launch(k_paged_attn<D, HALF>, dim3(sp.blocks), dim3(PA_THREADS), smem, s, a, sp);
+    if (e != cudaSuccess || units <= 1) return e;
+    const int by_pair = (long long)a.rows * sp.pairs <= sp.blocks;
+    // warps a head: all 16 where few heads are to be joined, so that many pieces are added at once; fewer where
+    // blocks would outnumber two an SM
+    const int cut = by_pair ? a.rows * sp.pairs : sp.blocks, heads = std::min(group, PA_HEADS);
+    int per_head = JOIN_THREADS / 32;
+    while (per_head > 1 && (long long)cut * heads * per_head / (JOIN_THREADS / 32) > 2 * sm_count()) per_head /= 2;
+    const int heads_a_block = JOIN_THREADS / 32 / per_head;
+    return pdl_launch(k_paged_join<D, HALF>, dim3(cut, (heads + heads_a_block - 1) / heads_a_block), dim3(JOIN_THREADS), sums, s, a,
+                      sp, by_pair, per_head);
 }
 
 }  // namespace
