@@ -70,7 +70,7 @@ int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv, int64_t q
         q_stride < (long long)heads * cache->head_dim || q_stride % 8 || (rope && (rope_rows < 1 || !positions)) ||
         !(eps >= 0.f))
         return invalid("Invalid paged qkv arguments");
-    if ((long long)tokens * width / 8 > (long long)INT_MAX * 128) return invalid("Too many tokens in one paged qkv call");
+    if ((long long)tokens * (heads + 2 * cache->kv_heads) > INT_MAX / 2) return invalid("Too many tokens in one paged qkv call");
     if (!aligned16(qkv) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(rope) || !aligned16(q))
         return invalid("Paged qkv pointers must be 16-byte aligned");
     return launched(launch_paged_qkv({cache_args(cache), static_cast<const uint16_t*>(qkv), qkv_stride, tokens, heads,
