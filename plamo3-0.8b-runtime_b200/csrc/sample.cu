@@ -9,14 +9,19 @@
 //
 // A cluster of up to 8 blocks takes a row: each keeps its slice of the logits in shared memory after one
 // read from global memory, and sums and histograms are exchanged through distributed shared memory, one
-// cluster barrier each. A threshold takes a histogram over 512 equal steps of (max - x), which spreads
-// the many near-equal logits that bins by bits of x would pile onto a few addresses. When at most 1024 ids
-// lie up to the step where k or p is reached (nearly always: what is kept is a small head of the vocabulary)
-// they are sent to the first block, which sorts them and finishes the row alone. Else the threshold is
-// narrowed down by histograms over the keys inside the step, and all blocks finish the row.
-// What cannot be kept is skipped before its exponential is taken: w = 0 beyond 27.8 T, and under top-p what
-// V times over would not fill the part that may be left out. Bound by instructions (an exponential an id
-// at least, unless top-k comes first) for many rows, by the cluster barriers for one.
+// cluster barrier each. What is kept is nearly always a small head of the vocabulary, so the aim is to name a
+// superset of it of at most 1024 ids, which the first block sorts and finishes alone:
+// - under top-k, the values from the j-th largest of the warps' maxima up: for k up to half the warps j = k, as
+//   k values are at least that large; for k up to twice the warps the j that leaves a quarter more than k if large
+//   values lie anywhere (n ids spread over N warps miss N e^{-n/N} of them), and k are counted. Else, and when
+//   that fails, those up to the step of a histogram where k is reached;
+// - under top-p, the values within 8.3 T of the top (there, one in 4000 as likely), listed in the pass that adds up all weights. When those do not
+//   hold p or are too many, a histogram of what could be kept at all (what V times over would fit into the part
+//   left out cannot) gives the step where p is reached. Histograms have 256 equal steps of (max - x), which spreads
+//   the many near-equal logits that bins by bits of x would pile onto a few addresses.
+// A larger superset has its threshold narrowed down by histograms over the keys inside the step, and all
+// blocks finish the row. w = 0 beyond 27.8 T. Bound by instructions (an exponential an id at least, unless top-k
+// comes first) for many rows, by the cluster barriers for one.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -33,8 +38,9 @@ namespace cg = cooperative_groups;
 
 constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
-constexpr int BINS = SAMPLE_THREADS;     // one bin a thread
+constexpr int BINS = 256;
 constexpr int LIST = 1024;               // ids that the first block can finish alone
+constexpr int FEW = 128;                 // ids that are compared each with each rather than sorted
 constexpr int MAX_CLUSTER = 8;
 constexpr int SLICE_BYTES = 128 * 1024;  // most of a slice kept in shared memory; the rest is read again
 constexpr float SPAN = 27.8f;            // 2^40 exp(-27.8) < 1
@@ -139,21 +145,24 @@ struct Pair {
 
 struct Shared {
     u64 hist[2][BINS];  // two, used in turn: one may still be read by other blocks while the next fills
-    uint32_t members[2][BINS];      // of a histogram of weights: how many values
     Pair exchange[4][MAX_CLUSTER];  // likewise; [i][c] is written by block c
     static_assert(LIST == 2 * SAMPLE_THREADS, "two entries a thread");
-    u64 list[LIST];     // the first block's: ~key << 32 | id, so ascending order is what ties need
-    uint32_t listed;
+    u64 list[LIST];     // ~key << 32 | id, so ascending order is what ties need; the first block's takes in all
+    u64 inbox[LIST];    // of the first block: an equal share for every block of the cluster; later a shorter list
+    uint32_t listed, counts[MAX_CLUSTER];
+    u64 few[FEW];       // weights of listed ids
+    float tops[MAX_CLUSTER * SAMPLE_WARPS];  // every warp's largest value
+    float least_top;
     Pair warp_pairs[SAMPLE_WARPS];
     u64 scan[SAMPLE_WARPS];
-    // a histogram's answer: the bin, the amount before it, the amount in it, the values up to and in it
-    u64 bin, before, amount, upto;
+    // a histogram's answer: the bin, the amount before it, the amount in it
+    u64 bin, before, amount;
 };
 
 template <int TYPE>
 struct Row {
     typedef typename Logit<TYPE>::raw raw;
-    static constexpr int VEC = 16 / sizeof(raw);
+    static constexpr int VEC = 16 / sizeof(raw), KS = Logit<TYPE>::KEY_SHIFT;
     cg::cluster_group cluster = cg::this_cluster();
     Shared& sh;
     raw* slice;           // the block's slice, `cached` values of it
@@ -162,7 +171,7 @@ struct Row {
     int lead;             // the row begins `lead` values after a 16-byte boundary: value j is id j - lead
     int begin, length, cached;  // the block's values [begin, begin + length)
     int mine0, mine1;     // this thread's values, from begin
-    int turn = 0, hist_turn = 0;
+    int turn = 0, hist_turn = 1;
     float top;
     Likelihood like;
 
@@ -240,61 +249,48 @@ struct Row {
         return before + x - v;
     }
 
-    // The same for a team of threads: one warp or the block.
-    template <int TEAM>
-    __device__ __forceinline__ void team_sync() {
-        if (TEAM == 32) __syncwarp();
-        else __syncthreads();
-    }
-    template <int TEAM>
-    __device__ __forceinline__ Pair team_add(Pair v) {
-        if (TEAM == 32) return Pair{warp_add(v.a), warp_add(v.b)};
-        return block_add(v);
-    }
-    template <int TEAM>
-    __device__ __forceinline__ u64 team_scan(u64 v) {
-        if (TEAM == 32) return warp_scan(v) - v;
-        return block_scan(v);
-    }
-
-    // One histogram over the cluster. classify(x) gives a value's bin (larger values in lower bins) or -1; an
-    // entry counts 1, or its weight. Finds the first bin at which `base` and the amounts up to it reach `need`
-    // (left in sh.bin / before / amount / upto); false when they do not.
-    template <bool WEIGHTS, typename F>
-    __device__ __forceinline__ bool histogram(F classify, u64 base, u64 need) {
-        u64* const hist = sh.hist[hist_turn & 1];
-        uint32_t* const counts = sh.members[hist_turn++ & 1];
-        if (WEIGHTS) hist[threadIdx.x] = 0;
-        counts[threadIdx.x] = 0;
+    // Histograms over the cluster, of numbers or of weights: cleared, filled by every block (larger values in
+    // lower bins), and after a cluster barrier read by find().
+    __device__ __forceinline__ void clear() {
+        hist_turn++;
+        if (threadIdx.x < BINS) sh.hist[hist_turn & 1][threadIdx.x] = 0;
         if (threadIdx.x == 0) sh.bin = BINS;
         __syncthreads();
-        each(classify, [&](float x, int bin, int) {
-            if (bin < 0) return;
-            if (WEIGHTS) {
-                const u64 w = weight(x);
-                if (!w) return;
-                atomicAdd(hist + bin, w);
-            }
-            atomicAdd(counts + bin, 1u);
-        });
-        cluster.sync();
-        u64 sum = 0, count = 0;
+    }
+    template <bool WEIGHTS>
+    __device__ __forceinline__ void put(int bin, u64 w) {
+        u64* const at = sh.hist[hist_turn & 1] + bin;
+        if (WEIGHTS) atomicAdd(at, w);
+        else atomicAdd(reinterpret_cast<uint32_t*>(at), 1u);  // below 2^32: the lower half is enough
+    }
+    // The first bin at which `base` and the amounts up to it reach `need` (left in sh.bin / before / amount); false
+    // when they do not.
+    __device__ __forceinline__ bool find(u64 base, u64 need) {
+        u64 sum = 0;
+        if (threadIdx.x < BINS) {
 #pragma unroll
-        for (int c = 0; c < MAX_CLUSTER; c++) {  // all reads in flight together
-            if (c >= ranks) continue;
-            if (WEIGHTS) sum += cluster.map_shared_rank(hist, c)[threadIdx.x];
-            count += cluster.map_shared_rank(counts, c)[threadIdx.x];
+            for (int c = 0; c < MAX_CLUSTER; c++)  // all reads in flight together
+                if (c < ranks) sum += cluster.map_shared_rank(sh.hist[hist_turn & 1], c)[threadIdx.x];
         }
-        if (!WEIGHTS) sum = count;
-        const u64 before = base + block_scan(sum), counted = WEIGHTS ? block_scan(count) : before - base;
+        const u64 before = base + block_scan(sum);
         if (before < need && need <= before + sum) {
             sh.bin = threadIdx.x;
             sh.before = before;
             sh.amount = sum;
-            sh.upto = counted + count;
         }
         __syncthreads();
         return sh.bin < BINS;
+    }
+    // All three; classify(x) gives a value's bin or -1.
+    template <bool WEIGHTS, typename F>
+    __device__ __forceinline__ bool histogram(F classify, u64 base, u64 need) {
+        clear();
+        each(classify, [&](float x, int bin, int) {
+            const u64 w = WEIGHTS && bin >= 0 ? weight(x) : 1ull;
+            if (bin >= 0 && w) put<WEIGHTS>(bin, w);
+        });
+        cluster.sync();
+        return find(base, need);
     }
 
     // Steps of (max - x) up to `limit` below the largest; -1 beyond it.
@@ -305,97 +301,207 @@ struct Row {
             if (!(x > -INFINITY) || d > limit) return -1;
             return min(int(d * step), BINS - 1);
         }
+        // bounds of the values in a bin, wider than the two roundings above
+        __device__ __forceinline__ float largest(int bin) const {
+            return __double2float_ru(double(top) - (bin ? bin / double(step) : 0.0) * (1.0 - 1e-6));
+        }
+        __device__ __forceinline__ float least(int bin) const {
+            if (top == INFINITY) return top;
+            return __double2float_rd(double(top) - (bin == BINS - 1 ? double(limit) : (bin + 1) / double(step)) * (1.0 + 1e-6));
+        }
     };
 
-    // Sends every value in a step up to `bin` to the first block's list; the number sent by the whole cluster.
-    __device__ __forceinline__ int gather(const Steps& steps, int bin, uint32_t least_key) {
-        uint32_t* const count = cluster.map_shared_rank(&sh.listed, 0);
-        u64* const list = cluster.map_shared_rank(sh.list, 0);
-        each([&](float x) { return key(x) < least_key ? -1 : steps(x); },
-             [&](float x, int b, int i) {
-                 if (b < 0 || b > bin) return;
-                 const uint32_t n = atomicAdd(count, 1u);
-                 if (n < LIST) list[n] = u64(~key(x)) << 32 | uint32_t(begin + i - lead);
+    __device__ __forceinline__ void start_list() {
+        if (threadIdx.x == 0) sh.listed = 0;
+        __syncthreads();
+    }
+    __device__ __forceinline__ void add_to_list(float x, int i) {
+        const uint32_t n = atomicAdd(&sh.listed, 1u);
+        if (n < LIST) sh.list[n] = u64(~key(x)) << 32 | uint32_t(begin + i - lead);
+    }
+    // Brings the blocks' lists together in the first block; the number of ids, or -1 when they do not fit. Each block
+    // leaves up to its share in the first block's inbox before the barrier that makes the numbers known; only when
+    // some block has more does it take a second barrier. Two sums over the cluster travel along.
+    __device__ __forceinline__ int deliver(Pair& sums) {
+        __syncthreads();
+        const uint32_t mine = sh.listed, share = LIST / ranks;
+        if (rank) {
+            u64* const to = cluster.map_shared_rank(sh.inbox, 0) + rank * share;
+            for (uint32_t i = threadIdx.x; i < min(mine, share); i += SAMPLE_THREADS) to[i] = sh.list[i];
+        }
+        if (threadIdx.x < ranks) *cluster.map_shared_rank(sh.counts + rank, threadIdx.x) = mine;
+        Pair unused;
+        sums = exchange(sums, unused);
+        uint32_t total = 0, before = 0;
+        bool over = false;
+        for (int c = 0; c < ranks; c++) {
+            const uint32_t n = sh.counts[c];
+            over |= n > share;
+            before += c < rank ? n : 0u;
+            total += n;
+        }
+        if (total > LIST) return -1;
+        if (over) {
+            if (rank) {
+                u64* const to = cluster.map_shared_rank(sh.list, 0) + before;
+                for (uint32_t i = threadIdx.x; i < mine; i += SAMPLE_THREADS) to[i] = sh.list[i];
+            }
+            cluster.sync();
+        } else if (rank == 0) {
+            uint32_t at = mine;
+            for (int c = 1; c < ranks; c++) {
+                const uint32_t n = sh.counts[c];
+                if (threadIdx.x < n) sh.list[at + threadIdx.x] = sh.inbox[c * share + threadIdx.x];  // n <= share <= 512
+                at += n;
+            }
+            __syncthreads();
+        }
+        return int(total);
+    }
+    // Lists the values x >= from, down to `far` below the top.
+    __device__ __forceinline__ int gather(float from, float far) {
+        start_list();
+        each([&](float x) { return x >= from && x > -INFINITY && !(top - x > far); },
+             [&](float x, bool wanted, int i) {
+                 if (wanted) add_to_list(x, i);
              });
-        cluster.sync();
-        return rank == 0 ? int(sh.listed) : 0;
+        Pair none{0, 0};
+        return deliver(none);
     }
 
-    // Sorts the list's first n entries ascending (n a power of two, at most 2 * TEAM): bitonic, in shared memory.
-    template <int TEAM>
-    __device__ __forceinline__ void sort_list(int n) {
+    // Sorts the list's first n entries ascending (n a power of two): bitonic, in shared memory.
+    __device__ __forceinline__ void sort_list(u64* list, int n) {
         for (int size = 2; size <= n; size *= 2)
             for (int gap = size / 2; gap > 0; gap /= 2) {
-                team_sync<TEAM>();
+                __syncthreads();
                 if (threadIdx.x < n / 2) {
                     const int i = threadIdx.x, lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
-                    const u64 a = sh.list[lo], b = sh.list[hi];
+                    const u64 a = list[lo], b = list[hi];
                     if ((a > b) == ((lo & size) == 0)) {
-                        sh.list[lo] = b;
-                        sh.list[hi] = a;
+                        list[lo] = b;
+                        list[hi] = a;
                     }
                 }
             }
-        team_sync<TEAM>();
+        __syncthreads();
     }
 
-    // The row's last steps, by the first TEAM threads of the first block (its first warp, or all): n ids on the
-    // list, n <= 2 * TEAM, hold everything that can be kept. run_known: the weight that top-p is a share of (0: that
-    // of the first k listed ones).
-    template <int TEAM>
+    // The row's last steps, by the first block alone: n ids on the list hold everything that can be kept. run_known: the
+    // weight that top-p is a share of (0: that of the first k listed ones).
     __device__ __forceinline__ void finish_list(const SampleArgs& a, int r, int n, int k, u64 p24, u64 least, u64 m, u64 run_known) {
-        constexpr int KS = Logit<TYPE>::KEY_SHIFT;
+        if (rank != 0) return;
+        u64* list = sh.list;
+        const bool nucleus = p24 < (1ull << 24);
+        if (n > FEW && (k < n || (nucleus && run_known))) {
+            // a shorter list: the values up to the step where k, or p, is reached
+            const Steps steps{top, like.T * SPAN, float(BINS) / (like.T * SPAN)};
+            clear();
+            if (threadIdx.x == 0) sh.listed = 0;
+            for (int i = threadIdx.x; i < n; i += SAMPLE_THREADS) {
+                const float x = key_value<KS>(uint32_t(~list[i] >> 32));
+                const u64 w = k < n ? 1ull : weight(x);
+                if (w) put<true>(steps(x), w);
+            }
+            __syncthreads();
+            const u64 need = k < n ? u64(k) : max(share(p24, run_known, true), 1ull);
+            const u64 sum = threadIdx.x < BINS ? sh.hist[hist_turn & 1][threadIdx.x] : 0ull, before = block_scan(sum);
+            if (before < need && need <= before + sum) sh.bin = threadIdx.x;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += SAMPLE_THREADS) {
+                const u64 entry = list[i];
+                if (u64(steps(key_value<KS>(uint32_t(~entry >> 32)))) <= sh.bin) sh.inbox[atomicAdd(&sh.listed, 1u)] = entry;
+            }
+            __syncthreads();
+            list = sh.inbox;
+            n = int(sh.listed);
+        }
+        if (n <= FEW) finish_few(list, a, r, n, k, p24, least, m, run_known);
+        else finish_many(list, a, r, n, k, p24, least, m, run_known);
+    }
+    // By sorting, two neighbouring entries a thread.
+    __device__ __forceinline__ void finish_many(u64* list, const SampleArgs& a, int r, int n, int k, u64 p24, u64 least, u64 m,
+                                                u64 run_known) {
         const int t = threadIdx.x;
         int size = 2;
         while (size < n) size *= 2;
-        for (int i = n + t; i < size; i += TEAM) sh.list[i] = ~0ull;
-        sort_list<TEAM>(size);
-        u64 w[2];  // two neighbouring entries a thread
+        for (int i = n + t; i < size; i += SAMPLE_THREADS) list[i] = ~0ull;
+        sort_list(list, size);
+        u64 w[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const int i = 2 * t + e;
-            w[e] = i < n && i < k ? weight(key_value<KS>(uint32_t(~sh.list[i] >> 32))) : 0ull;
+            w[e] = i < n && i < k ? weight(key_value<KS>(uint32_t(~list[i] >> 32))) : 0ull;
         }
-        const bool nucleus = p24 < (1ull << 24);
-        const u64 before = team_scan<TEAM>(w[0] + w[1]);
-        if (nucleus) {
-            const u64 run = run_known ? run_known : team_add<TEAM>({w[0] + w[1], 0}).a, need = max(share(p24, run, true), 1ull);
+        const u64 before = block_scan(w[0] + w[1]);
+        if (p24 < (1ull << 24)) {
+            const u64 run = run_known ? run_known : block_add({w[0] + w[1], 0}).a, need = max(share(p24, run, true), 1ull);
             if (before + w[0] >= need) w[1] = 0;
             if (before >= need) w[0] = 0;
         }
         if (w[0] < least) w[0] = 0;
         if (w[1] < least) w[1] = 0;
-        const Pair total = team_add<TEAM>({w[0] + w[1], u64((w[0] != 0) + (w[1] != 0))});
+        const Pair total = block_add({w[0] + w[1], u64((w[0] != 0) + (w[1] != 0))});
         // the kept ones are the first total.b; now in index order, each with its key
         const int kept = int(total.b);
         size = 2;
         while (size < kept) size *= 2;
         u64 entry[2];
 #pragma unroll
-        for (int e = 0; e < 2; e++) entry[e] = 2 * t + e < kept ? sh.list[2 * t + e] : 0ull;
-        team_sync<TEAM>();
+        for (int e = 0; e < 2; e++) entry[e] = 2 * t + e < kept ? list[2 * t + e] : 0ull;
+        __syncthreads();
 #pragma unroll
         for (int e = 0; e < 2; e++)
-            if (2 * t + e < size) sh.list[2 * t + e] = 2 * t + e < kept ? entry[e] << 32 | uint32_t(~entry[e] >> 32) : ~0ull;
-        sort_list<TEAM>(size);
+            if (2 * t + e < size) list[2 * t + e] = 2 * t + e < kept ? entry[e] << 32 | uint32_t(~entry[e] >> 32) : ~0ull;
+        sort_list(list, size);
 #pragma unroll
-        for (int e = 0; e < 2; e++) w[e] = 2 * t + e < kept ? weight(key_value<KS>(uint32_t(sh.list[2 * t + e]))) : 0ull;
+        for (int e = 0; e < 2; e++) w[e] = 2 * t + e < kept ? weight(key_value<KS>(uint32_t(list[2 * t + e]))) : 0ull;
         const u64 target = share(m, total.a, false);
-        u64 upto = team_scan<TEAM>(w[0] + w[1]);
+        u64 upto = block_scan(w[0] + w[1]);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             if (upto <= target && target < upto + w[e]) {
-                a.ids[r] = int(sh.list[2 * t + e] >> 32);
+                a.ids[r] = int(list[2 * t + e] >> 32);
                 if (a.logprobs) a.logprobs[r] = log_share(w[e], total.a);
             }
             upto += w[e];
         }
         if (t == 0 && a.kept) a.kept[r] = kept;
     }
-    __device__ __forceinline__ void finish_listed(const SampleArgs& a, int r, int n, int k, u64 p24, u64 least, u64 m, u64 run_known) {
-        if (rank != 0) return;
-        if (n > 64) finish_list<SAMPLE_THREADS>(a, r, n, k, p24, least, m, run_known);
-        else if (threadIdx.x < 32) finish_list<32>(a, r, n, k, p24, least, m, run_known);
+    // Places and running weights of at most FEW ids by comparing each with each, four threads (or eight) an id: fewer
+    // dependent steps than a sort.
+    __device__ __forceinline__ void finish_few(const u64* list, const SampleArgs& a, int r, int n, int k, u64 p24, u64 least, u64 m,
+                                               u64 run_known) {
+        const int team = n <= FEW / 2 ? 8 : 4, i = threadIdx.x / team, part = threadIdx.x % team;
+        const u64 mine = i < n ? list[i] : ~0ull;
+        auto team_add = [&](u64 v) {
+            for (int o = 1; o < team; o *= 2) v += __shfl_xor_sync(FULL_MASK, v, o);
+            return v;
+        };
+        uint32_t place = 0;
+        for (int j = part; j < n; j += team) place += list[j] < mine;
+        place = uint32_t(team_add(place));
+        u64 w = i < n && place < uint32_t(k) ? weight(key_value<KS>(uint32_t(~mine >> 32))) : 0ull;
+        if (p24 < (1ull << 24)) {
+            if (part == 0 && i < FEW) sh.few[i] = w;
+            const u64 run = run_known ? run_known : block_add({part == 0 ? w : 0ull, 0}).a, need = max(share(p24, run, true), 1ull);
+            __syncthreads();
+            u64 before = 0;
+            for (int j = part; j < n; j += team) before += list[j] < mine ? sh.few[j] : 0ull;
+            if (team_add(before) >= need) w = 0;
+            __syncthreads();
+        }
+        if (w < least) w = 0;
+        if (part == 0 && i < FEW) sh.few[i] = w;
+        const Pair total = block_add({part == 0 ? w : 0ull, part == 0 && w});
+        const u64 target = share(m, total.a, false);
+        u64 upto = 0;  // kept weight of the lower ids
+        for (int j = part; j < n; j += team) upto += uint32_t(list[j]) < uint32_t(mine) ? sh.few[j] : 0ull;
+        upto = team_add(upto);
+        if (part == 0 && upto <= target && target < upto + w) {
+            a.ids[r] = int(uint32_t(mine));
+            if (a.logprobs) a.logprobs[r] = log_share(w, total.a);
+        }
+        if (threadIdx.x == 0 && a.kept) a.kept[r] = int(total.b);
     }
 
     // After histogram() over `steps`: the key at which the amounts of the values, from the largest down, reach
@@ -405,14 +511,9 @@ struct Row {
                                            u64& amount) {
         const int bin = int(sh.bin);
         u64 base = sh.before;
-        // keys that the step can hold: its bounds, widened by more than the two roundings of `steps`
-        const double low = bin == BINS - 1 ? double(steps.limit) : (bin + 1) / double(steps.step),
-                     high = bin ? bin / double(steps.step) : 0.0;
-        uint32_t khi = key(__double2float_ru(double(top) - high * (1.0 - 1e-6)));
-        uint32_t klo = key(__double2float_rd(double(top) - low * (1.0 + 1e-6)));
-        if (top == INFINITY) khi = klo = key(top);
+        uint32_t khi = key(steps.largest(bin)), klo = key(steps.least(bin));
         while (true) {
-            const int bits = 32 - __clz(khi - klo), shift = max(bits - 9, 0);
+            const int bits = 32 - __clz(khi - klo), shift = max(bits - 8, 0);
             __syncthreads();  // the answer before has been read
             auto fine = [&](float x) -> int {
                 const uint32_t k = key(x);
@@ -493,19 +594,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
         }
     }
     top = warp_max(top);
-    Pair unused;
-    {
-        Pair* const places = shared.exchange[row.turn++ & 3];
-        if ((t & 31) == 0) shared.scan[t >> 5] = __float_as_uint(top);
-        if (t == 0) shared.listed = 0;
-        __syncthreads();
-        top = warp_max(t % 32 < SAMPLE_WARPS ? __uint_as_float(uint32_t(shared.scan[t % 32])) : -INFINITY);
-        row.cluster.barrier_wait();
-        if (t < row.ranks) row.cluster.map_shared_rank(places + row.rank, t)->a = __float_as_uint(top);
-        row.cluster.sync();
-        const int lane = t & 31;
-        top = warp_max(lane < row.ranks ? __uint_as_float(uint32_t(places[lane].a)) : -INFINITY);
-    }
+    if ((t & 31) == 0) shared.scan[t >> 5] = __float_as_uint(top);
+    __syncthreads();
+    row.cluster.barrier_wait();
+    const int warps = row.ranks * SAMPLE_WARPS;
+    if (t < warps)
+        row.cluster.map_shared_rank(shared.tops, t / SAMPLE_WARPS)[row.rank * SAMPLE_WARPS + t % SAMPLE_WARPS] =
+            __uint_as_float(uint32_t(shared.scan[t % SAMPLE_WARPS]));
+    row.cluster.sync();
+    for (int i = t & 31; i < warps; i += 32) top = fmaxf(top, shared.tops[i]);
+    top = warp_max(top);
     row.top = top;
     row.like.set(top, T);
 
@@ -518,11 +616,33 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     // kept: keys above `edge`, and the first `ties` (in index order) of the `at_edge` values at it
     uint32_t edge = 0;
     u64 ties = 0, at_edge = 0, before, amount;
+    if (k <= 2 * warps) {
+        const int j = k <= warps / 2 ? k : min(warps, int(ceilf(warps * (1.f - __expf(-(1.25f * k + 24.f) / warps)))));
+        // the j-th largest of the warps' maxima: a quarter of them for each of four threads to compare with
+        const int i = t / 4;
+        int above = 0;
+        if (i < warps)
+#pragma unroll 8
+            for (int o = t & 3; o < warps; o += 4)
+                above += shared.tops[o] > shared.tops[i] || (shared.tops[o] == shared.tops[i] && o < i);
+        above += __shfl_xor_sync(FULL_MASK, above, 1);
+        above += __shfl_xor_sync(FULL_MASK, above, 2);
+        if (i < warps && above == j - 1) shared.least_top = shared.tops[i];
+        __syncthreads();
+        const float from = shared.least_top;
+        const int n = row.gather(from, far);
+        // fewer than k are enough where none of the others weighs anything: nothing further down was left out
+        if (n >= k || (n > 0 && (from == -INFINITY || top - from > far))) {
+            row.finish_list(a, r, n, k, p24, least, m, 0);
+            return;
+        }
+    }
     if (k < V) {
         const Steps steps{top, far, float(BINS) / far};
         if (row.template histogram<false>(steps, 0, k)) {
-            if (shared.upto <= LIST) {
-                row.finish_listed(a, r, row.gather(steps, int(shared.bin), 0u), k, p24, least, m, 0);
+            const int n = shared.before + shared.amount <= LIST ? row.gather(steps.least(int(shared.bin)), far) : -1;
+            if (n >= 0) {
+                row.finish_list(a, r, n, k, p24, least, m, 0);
                 return;
             }
             row.template narrow<false>(steps, k, 0u, edge, before, amount);
@@ -531,22 +651,44 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
         }
     }
     if (nucleus) {
-        Pair w{0, 0};
-        auto add = [&](float, float e, int) { w.a += e >= LEAST ? fixed(e) : 0ull; };
+        // all weights, those near the top, and a list of the latter
+        const float near = far * 0.3f;
+        u64 all_weight = 0, near_weight = 0;
+        row.start_list();
+        auto add = [&](float x, float e, int i) {
+            if (e >= LEAST) {
+                const u64 f = fixed(e);
+                all_weight += f;
+                if (!(top - x > near)) {
+                    near_weight += f;
+                    row.add_to_list(x, i);
+                }
+            }
+        };
         if (edge) row.each([&](float x) { return x > -INFINITY && row.key(x) >= edge ? row.like(x) : 0.f; }, add);
         else row.each(row.like, add);
-        const u64 one = ties < at_edge ? row.weight(key_value<KS>(edge)) : 0ull;
-        const u64 run = row.exchange(row.block_add(w), unused).a - (at_edge - ties) * one;
-        const u64 need = max(share(p24, run, true), 1ull);
+        Pair sums = row.block_add({all_weight, near_weight});
+        const int n = row.deliver(sums);
+        const u64 cut_off = ties < at_edge ? (at_edge - ties) * row.weight(key_value<KS>(edge)) : 0ull;
+        const u64 run = sums.a - cut_off, need = max(share(p24, run, true), 1ull);
+        if (n >= 0 && run && sums.b >= need && !cut_off) {
+            row.finish_list(a, r, n, k, p24, least, m, run);
+            return;
+        }
         // an id whose weight V times over fits into what may be left out is left out itself
         const u64 small = (run - min(need, run)) / u64(V);
         const float limit = small > 1 ? fminf(far, T * (log2f(1099511627776.0f / float(small)) * 0.6931472f) * 1.0001f + 1e-6f * T) : far;
         const Steps steps{top, limit, float(BINS) / limit};
         auto within = [&](float x) -> int { return row.key(x) < edge ? -1 : steps(x); };
-        if (run && row.template histogram<true>(within, 0, need)) {
-            if (shared.upto <= LIST && ties == at_edge) {  // top-k has not cut through equal values
-                row.finish_listed(a, r, row.gather(steps, int(shared.bin), edge), k, p24, least, m, run);
-                return;
+        const bool found = run && row.template histogram<true>(within, 0, need);
+        if (found) {
+            if (ties == at_edge) {  // top-k has not cut through equal values
+                const float from = steps.least(int(shared.bin));
+                const int n = row.gather(edge ? fmaxf(from, key_value<KS>(edge)) : from, far);
+                if (n >= 0) {
+                    row.finish_list(a, r, n, k, p24, least, m, run);
+                    return;
+                }
             }
             uint32_t cut = edge;
             row.template narrow<true>(steps, need, edge, cut, before, amount);
