@@ -174,7 +174,7 @@ PLAMO_API int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv,
  * row_start NULL: request r's query is row r of q [q_rows][heads][head_dim] (q_stride elements apart), and
  * q_rows >= rows. Else it is row row_start[r + 1] - 1 (the request's last packed token of
  * plamo_k_paged_plan), and requests without a token are skipped. heads: a multiple of kv_heads, at most 256.
- *   out = sum_j softmax_j(scale * q.k_j) v_j in fp32 (the probabilities enter the products as hi + lo pairs
+ *   out = sum_j softmax_j(scale * q.k_j) v_j (scale > 0) in fp32 (the probabilities enter the products as hi + lo pairs
  *   of the 16-bit type), rounded once; lse (may be NULL, [q_rows][heads] fp32) = ln sum_j exp(scale * q.k_j).
  * A request that sees no key, or whose scores are all -inf, gets zeros and lse -inf. Query rows that belong
  * to no request are not written. `workspace`: 16-byte aligned device memory of at least

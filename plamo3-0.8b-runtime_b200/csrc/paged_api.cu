@@ -88,7 +88,7 @@ int plamo_k_paged_attention(const plamo_paged_cache* cache, const void* q, int64
     if (const char* fault = cache_fault(cache)) return invalid(fault);
     if (!q || !table || !lens || !out || rows < 1 || rows > PAGED_MAX_ROWS || q_rows < 1 || (!row_start && q_rows < rows) ||
         heads < 1 || heads > 256 || heads % cache->kv_heads || table_stride < 1 || max_len < 1 || max_len > (1 << 30) ||
-        max_len > (long long)table_stride * cache->page_size || window < 0 || !std::isfinite(scale) ||
+        max_len > (long long)table_stride * cache->page_size || window < 0 || !std::isfinite(scale) || !(scale > 0.f) ||
         q_stride < (long long)heads * cache->head_dim || out_stride < (long long)heads * cache->head_dim || q_stride % 8 ||
         out_stride % 8)
         return invalid("Invalid paged attention arguments");

@@ -14,8 +14,11 @@
 // Block. Four warps take every fourth 16-key tile of a stretch, each with its own running maximum, sum and
 // outputs and its own ring of tiles: no barrier inside the loop. A tile's keys and values are copied with
 // cp.async in an XOR-swizzled layout, so ldmatrix reads them without bank conflicts; the page lookup of a
-// tile runs one tile ahead of its copy. Keys outside the visible range or without a page are filled
-// with zeros and their scores replaced by -inf, so nothing stored there can reach a result.
+// tile runs one tile ahead of its copy. Tiles begin at positions that are multiples of 16, so where the
+// page size is one too a tile lies in one page and has one lookup; else each key has its own. Keys
+// outside the visible range or without a page are filled with zeros and their scores replaced by -inf, so
+// nothing stored there can reach a result.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,6 +32,8 @@
 namespace plamo {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int PA_THREADS = 128;
 constexpr int PA_WARPS = PA_THREADS / 32;
 constexpr int PA_HEADS = 16;  // query heads of a block: the MMA's rows
@@ -38,6 +43,11 @@ constexpr int PA_UNIT = 64;   // keys of a unit: one tile for each warp
 constexpr int PA_WHOLE = 256;
 // What beginning a request and head costs a block, in units: its share of the line is that much longer.
 constexpr int PA_BEGIN = 3;
+// A cluster takes a request and head where all clusters' blocks run at once and a block's share of the longest
+// request is at most this many keys: the first number always, the second when the blocks fill most SMs.
+constexpr int PA_CLUSTER = 8;
+constexpr int PA_SHARE = 264;
+constexpr int PA_SHARE_FULL = 640;
 constexpr int PA_MAX_BLOCKS = 592;
 constexpr int JOIN_THREADS = 512;
 // tiles in a warp's ring: 96 KB a block, two blocks an SM
@@ -47,11 +57,11 @@ constexpr int PA_STAGES = 384 / D;
 template <bool HALF>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if (HALF)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -63,6 +73,9 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     else
         asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // 16 bytes into shared memory, or zeros where there is nothing to read.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
@@ -123,61 +136,96 @@ constexpr float P_SHIFT = HALF ? 14.f : 0.f;
 // A maximum of -inf (nothing seen yet) is replaced by 0 where it is subtracted: e^{-inf - 0} = 0, not NaN.
 __device__ __forceinline__ float origin(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Adds one tile of 16 keys (at kt, values at vt) of which those in `mask` are visible.
+// Where a lane's ldmatrix and copy addresses lie in a tile, the same for every tile: the swizzle repeats every 8
+// chunks and every 8 rows, so four offsets and constants beside them are enough.
+template <int D>
+struct Offsets {
+    static constexpr int ROW = D * 2, CH = D / 8, RPS = 32 / CH, COPIES = 8 / RPS;  // rows a step of copies, steps of 8 rows
+    uint32_t key[4], value[4], copy[COPIES];
+    __device__ __forceinline__ Offsets() {
+        const int lane = threadIdx.x & 31;
+        // keys: lanes 0-7 / 8-15 address keys 0-7 at a k-step's first / second chunk, 16-31 keys 8-15 likewise
+        const int krow = (lane & 7) + ((lane >> 4) << 3), kchunk = (lane >> 3) & 1;
+        // values: lanes 0-15 address keys 0-15 of a chunk, lanes 16-31 those of the next
+        const int vrow = lane & 15, vchunk = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            key[i] = krow * ROW + (((2 * i + kchunk) ^ (krow & 7)) << 4);
+            value[i] = vrow * ROW + (((2 * i + vchunk) ^ (vrow & 7)) << 4);
+        }
+#pragma unroll
+        for (int i = 0; i < COPIES; i++) {
+            const int row = i * RPS + lane / CH;
+            copy[i] = row * ROW + (((lane % CH) ^ (row & 7)) << 4);
+        }
+    }
+};
+
+// Adds one tile of 16 keys (at kt, values behind them) of which those in `mask` are visible.
 template <int D, bool HALF>
-__device__ __forceinline__ void add_tile(Running<D>& run, const uint32_t (&qa)[D / 16][4], uint32_t kt, uint32_t vt,
+__device__ __forceinline__ void add_tile(Running<D>& run, const uint32_t (&qa)[D / 16][4], const Offsets<D>& off, uint32_t kt,
                                          uint32_t mask, float scale) {
-    const int lane = threadIdx.x & 31, tq = lane & 3;
-    float acc[2][4];
+    const int tq = threadIdx.x & 3;
+    // even and odd k-steps are added up apart: half the length of a chain of dependent MMAs
+    float acc[2][4], odd[2][4];
 #pragma unroll
     for (int n = 0; n < 2; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[n][i] = 0.f;
-    // lanes 0-7 / 8-15 address keys 0-7 at the k-step's first / second chunk, 16-31 keys 8-15 likewise
-    const int krow = (lane & 7) + ((lane >> 4) << 3), kchunk = (lane >> 3) & 1;
+        for (int i = 0; i < 4; i++) acc[n][i] = odd[n][i] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < D / 16; kk++) {
         uint32_t b[4];
-        ldsm4<false>(b, kt + krow * (D * 2) + (((2 * kk + kchunk) ^ (krow & 7)) << 4));
-        mma16816<HALF>(acc[0], qa[kk], b[0], b[1]);
-        mma16816<HALF>(acc[1], qa[kk], b[2], b[3]);
+        ldsm4<false>(b, kt + off.key[kk & 3] + (kk >> 2) * 128);
+        mma16816<HALF>(kk & 1 ? odd[0] : acc[0], qa[kk], b[0], b[1]);
+        mma16816<HALF>(kk & 1 ? odd[1] : acc[1], qa[kk], b[2], b[3]);
     }
 #pragma unroll
     for (int n = 0; n < 2; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            acc[n][i] = (mask >> (8 * n + 2 * tq + (i & 1))) & 1u ? acc[n][i] * scale : -INFINITY;
+        for (int i = 0; i < 4; i++) acc[n][i] += odd[n][i];
+    if (mask != 0xffffu) {
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (!((mask >> (8 * n + 2 * tq + (i & 1))) & 1u)) acc[n][i] = -INFINITY;
+    }
     uint32_t ph[4], pl[4];
+    float fade[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         float top = fmaxf(fmaxf(acc[0][2 * h], acc[0][2 * h + 1]), fmaxf(acc[1][2 * h], acc[1][2 * h + 1]));
         top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 1));
         top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 2));
-        const float m = fmaxf(run.m[h], top), base = origin(m);
-        const float fade = ex2(run.m[h] - base), origin_p = base - P_SHIFT<HALF>;
+        // the scale is positive: it does not change which score is the largest
+        const float m = fmaxf(run.m[h], top * scale), base = origin(m), origin_p = base - P_SHIFT<HALF>;
+        fade[h] = ex2(run.m[h] - base);
         run.m[h] = m;
         float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = ex2(acc[i >> 1][2 * h + (i & 1)] - origin_p);
-        run.l[h] = fmaf(run.l[h], fade, (p[0] + p[1]) + (p[2] + p[3]));
+        for (int i = 0; i < 4; i++) p[i] = ex2(fmaf(acc[i >> 1][2 * h + (i & 1)], scale, -origin_p));
+        run.l[h] = fmaf(run.l[h], fade[h], (p[0] + p[1]) + (p[2] + p[3]));
         split_pair<HALF>(p[0], p[1], ph[h], pl[h]);
         split_pair<HALF>(p[2], p[3], ph[2 + h], pl[2 + h]);
-#pragma unroll
-        for (int j = 0; j < D / 8; j++) {
-            run.o[j][2 * h] *= fade;
-            run.o[j][2 * h + 1] *= fade;
-        }
     }
-    // lanes 0-15 address keys 0-15 of a chunk, lanes 16-31 those of the next
-    const int vrow = lane & 15, vchunk = lane >> 4;
+    // most tiles leave every maximum where it was
+    if (__any_sync(FULL_MASK, fade[0] != 1.f || fade[1] != 1.f)) {
 #pragma unroll
-    for (int j = 0; j < D / 8; j += 2) {
-        uint32_t b[4];
-        ldsm4<true>(b, vt + vrow * (D * 2) + (((j + vchunk) ^ (vrow & 7)) << 4));
-        mma16816<HALF>(run.o[j], ph, b[0], b[1]);
-        mma16816<HALF>(run.o[j], pl, b[0], b[1]);
-        mma16816<HALF>(run.o[j + 1], ph, b[2], b[3]);
-        mma16816<HALF>(run.o[j + 1], pl, b[2], b[3]);
+        for (int j = 0; j < D / 8; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) run.o[j][i] *= fade[i >> 1];
+    }
+    const uint32_t vt = kt + PA_TILE * D * 2;
+#pragma unroll
+    for (int j = 0; j < D / 8; j += 4) {
+        uint32_t b[2][4];
+#pragma unroll
+        for (int g = 0; g < 2; g++) ldsm4<true>(b[g], vt + off.value[(j / 2 + g) & 3] + (j >> 3) * 128);
+        // the two products of an output are four MMAs apart
+#pragma unroll
+        for (int g = 0; g < 4; g++) mma16816<HALF>(run.o[j + g], ph, b[g >> 1][2 * (g & 1)], b[g >> 1][2 * (g & 1) + 1]);
+#pragma unroll
+        for (int g = 0; g < 4; g++) mma16816<HALF>(run.o[j + g], pl, b[g >> 1][2 * (g & 1)], b[g >> 1][2 * (g & 1) + 1]);
     }
 }
 
@@ -210,6 +258,8 @@ struct Split {
     int unit;       // keys of a unit
     int pairs;      // (KV head, block of 16 query heads) pairs of a request
     int per_kv;     // blocks of 16 query heads of a KV head
+    int group;      // query heads of a KV head
+    int page_shift; // log2 of the page size, -1 when it is no power of two
     int blocks;     // of k_paged_attn
 };
 
@@ -234,20 +284,29 @@ struct Line {
     __device__ __forceinline__ int begin_of(int block) const { return int(min((long long)block * per_block, (long long)total)); }
     __device__ __forceinline__ Place at(int x, int rows, int pairs) const {
         // the last request that begins at or before x
-        const int line = x / pairs;  // upto[mid] * pairs <= x
         int lo = 0, hi = rows - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (upto[mid] <= line) lo = mid;
+            if (upto[mid] * pairs <= x) lo = mid;
             else hi = mid - 1;
         }
         Place p;
         p.r = lo;
         p.length = upto[lo + 1] - upto[lo];
         const int inside = x - upto[lo] * pairs;
-        p.pair = inside / p.length;
+        p.pair = pairs == 1 ? 0 : inside / p.length;
         p.begin = x - (inside - p.pair * p.length);
         return p;
+    }
+};
+
+// What request r sees: keys [first, end). Units and tiles begin at `origin`, first rounded down to a tile.
+struct Seen {
+    int first, end, origin;
+    __device__ __forceinline__ Seen(const PagedAttnArgs& a, int r) {
+        end = min(max(a.lens[r], 0), a.max_len);
+        first = a.window > 0 ? max(0, end - a.window) : 0;
+        origin = first & ~(PA_TILE - 1);
     }
 };
 
@@ -260,8 +319,8 @@ __device__ __forceinline__ Line lay_out(const PagedAttnArgs& a, const Split& sp,
     const int per = (a.rows + THREADS - 1) / THREADS, r0 = min(t * per, a.rows), r1 = min(r0 + per, a.rows);
     int sum = 0;
     for (int r = r0; r < r1; r++) {
-        const int n = min(max(a.lens[r], 0), a.max_len), seen = a.window > 0 ? min(n, a.window) : n;
-        const int units = query_row(a, r) >= 0 ? (seen + sp.unit - 1) / sp.unit : 0;
+        const Seen seen(a, r);
+        const int units = query_row(a, r) >= 0 ? (seen.end - seen.origin + sp.unit - 1) / sp.unit : 0;
         const int places = units ? units + PA_BEGIN : 0;
         upto[r + 1] = places;
         sum += places;
@@ -289,151 +348,229 @@ __device__ __forceinline__ Line lay_out(const PagedAttnArgs& a, const Split& sp,
     return line;
 }
 
-template <int D, bool HALF>
+// A block's work on one request and KV head: keys [k0, k1) (k0 at a tile's beginning, nothing before `first` is
+// visible), of whose tiles warp number `warp` of `warps` takes every warps-th.
+struct Work {
+    int r, kv, head0, heads, qrow, first, k0, k1, warp, warps;
+};
+template <int D>
+constexpr int PA_PITCH = D + 8;  // a warp's outputs, a head a row: 8 floats further than a multiple of 32 banks
+
+// Runs the warp's tiles, and leaves the warps' outputs (relative to the block's maximum, PA_PITCH floats a head) in
+// the rings' place and their (maximum, sum) pairs in `stats`. Ends with a barrier.
+template <int D, bool HALF, bool ALIGNED>
+__device__ __forceinline__ void attend(const PagedAttnArgs& a, const Split& sp, const Work& w, uint8_t* smem,
+                                       float2 (*stats)[PA_HEADS]) {
+    constexpr int ROW = D * 2, TILE_BYTES = PA_TILE * ROW, CH = D / 8, S = PA_STAGES<D>, PITCH = PA_PITCH<D>;
+    static_assert(PA_HEADS * PITCH * 4 <= S * 2 * TILE_BYTES, "a warp's outputs fit in its ring");
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gq = lane >> 2, tq = lane & 3;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * S * 2 * TILE_BYTES;
+    const Offsets<D> at;
+    constexpr int RPS = Offsets<D>::RPS, COPIES = Offsets<D>::COPIES;
+    const int c = lane % CH, row0 = lane / CH;  // this lane copies chunk c of rows row0, row0 + RPS, ...
+    const int* table = a.table + size_t(w.r) * a.table_stride;
+    const int tiles = (w.k1 - w.k0 + PA_TILE - 1) / PA_TILE;
+    const int mine = tiles > w.warp ? (tiles - w.warp + w.warps - 1) / w.warps : 0;  // tiles w.warp, w.warp + w.warps, ...
+    const uint16_t* const keys = a.cache.keys + w.kv * a.cache.head_stride + c * 8;
+    const uint16_t* const values = a.cache.values + w.kv * a.cache.head_stride + c * 8;
+    const long long step = RPS * a.cache.token_stride;
+    auto page_index = [&](int key) { return sp.page_shift >= 0 ? key >> sp.page_shift : key / a.cache.page_size; };
+    // The page of the tile at key0 (ALIGNED), or of its key `lane % 16`; -1 outside the range.
+    auto page_of = [&](int key0) -> int {
+        const int key = key0 + (ALIGNED ? 0 : lane & 15);
+        return key < w.k1 ? __ldg(table + page_index(key)) : -1;
+    };
+    // Copies the tile at key0 to kt, values behind its keys; which of its keys are visible.
+    auto issue = [&](int key0, int page, uint32_t kt) -> uint32_t {
+        uint32_t mask = 0xffffu;
+        if (key0 < w.first || key0 + PA_TILE > w.k1)
+            mask = ((1u << min(w.k1 - key0, PA_TILE)) - 1u) & ~((1u << max(w.first - key0, 0)) - 1u);
+        const bool held = page >= 0 && page < a.cache.pages;
+        long long off = 0;  // of this lane's first row (ALIGNED), or of key `lane % 16`
+        if (ALIGNED) {
+            if (!held) mask = 0u;
+            off = page * a.cache.page_stride + (key0 - page_index(key0) * a.cache.page_size + row0) * a.cache.token_stride;
+        } else {
+            const int key = key0 + (lane & 15);
+            if (held) off = page * a.cache.page_stride + (key - page_index(key) * a.cache.page_size) * a.cache.token_stride;
+            mask &= __ballot_sync(FULL_MASK, held) & 0xffffu;
+        }
+        if (mask == 0xffffu) {
+#pragma unroll
+            for (int i = 0; i < PA_TILE / RPS; i++) {
+                const uint32_t dst = kt + at.copy[i % COPIES] + (i / COPIES) * 8 * ROW;
+                const long long from = ALIGNED ? off : __shfl_sync(FULL_MASK, off, i * RPS + row0);
+                copy16(dst, keys + from);
+                copy16(dst + TILE_BYTES, values + from);
+                if (ALIGNED) off += step;
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < PA_TILE / RPS; i++) {
+                const int row = i * RPS + row0;
+                const uint32_t dst = kt + row * ROW + ((c ^ (row & 7)) << 4);
+                const long long from = ALIGNED ? off : __shfl_sync(FULL_MASK, off, row);
+                const bool valid = mask >> row & 1u;
+                copy16(dst, valid ? keys + from : a.cache.keys, valid);
+                copy16(dst + TILE_BYTES, valid ? values + from : a.cache.values, valid);
+                if (ALIGNED) off += step;
+            }
+        }
+        return mask;
+    };
+    const int stride = w.warps * PA_TILE;
+    int key0 = w.k0 + w.warp * PA_TILE, ahead = key0;  // the next tile to copy, and to look up
+    int pages[S];  // the lookups of the next tiles to copy, the ring's first ones together
+#pragma unroll
+    for (int i = 0; i < S; i++, ahead += stride) pages[i] = page_of(ahead);
+    // the queries wait in the ring's last place until it is needed
+    const uint32_t qt = ring + (S - 1) * 2 * TILE_BYTES;
+    const uint16_t* const q = a.q + w.qrow * a.q_stride + w.head0 * D + c * 8;
+    if (mine)
+#pragma unroll
+        for (int i = 0; i < PA_TILE / RPS; i++) {
+            const int row = i * RPS + row0;
+            copy16(qt + at.copy[i % COPIES] + (i / COPIES) * 8 * ROW, row < w.heads ? q + row * D : a.q, row < w.heads);
+        }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    uint32_t qa[D / 16][4];
+    Running<D> run;
+    run.clear();
+    // tile j is copied while tile j - (S - 1) is worked on
+    uint32_t masks[S], to = ring, from = ring;
+    const uint32_t ring_end = ring + S * 2 * TILE_BYTES;
+#pragma unroll
+    for (int i = 0; i < S; i++) masks[i] = 0u;
+#pragma unroll 1
+    for (int j = 0; j < mine + S - 1; j++) {
+        if (j == S - 1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+            __syncwarp();
+            // the heads are addressed as the values' keys are
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) ldsm4<false>(qa[kk], qt + at.value[kk & 3] + (kk >> 2) * 128);
+            __syncwarp();
+        }
+        masks[S - 1] = j < mine ? issue(key0, pages[0], to) : 0u;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        key0 += stride;
+        to = to + 2 * TILE_BYTES == ring_end ? ring : to + 2 * TILE_BYTES;
+#pragma unroll
+        for (int i = 0; i < S - 1; i++) pages[i] = pages[i + 1];
+        pages[S - 1] = page_of(ahead);
+        ahead += stride;
+        if (j >= S - 1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+            __syncwarp();
+            add_tile<D, HALF>(run, qa, at, from, masks[0], a.scale_log2);
+            __syncwarp();  // the tile has been read: the next copy may overwrite it
+            from = from + 2 * TILE_BYTES == ring_end ? ring : from + 2 * TILE_BYTES;
+        }
+#pragma unroll
+        for (int i = 0; i < S - 1; i++) masks[i] = masks[i + 1];
+    }
+    // join the warps
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 1);
+        run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 2);
+        if (tq == 0) stats[warp][gq + 8 * h] = make_float2(run.m[h], run.l[h]);
+    }
+    __syncthreads();  // every warp is done with its ring
+    float* const mid = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][gq + 8 * h].x);
+        const float f = ex2(run.m[h] - origin(m));
+#pragma unroll
+        for (int j = 0; j < D / 8; j++)
+            *reinterpret_cast<float2*>(mid + (warp * PA_HEADS + gq + 8 * h) * PITCH + j * 8 + 2 * tq) =
+                make_float2(run.o[j][2 * h] * f, run.o[j][2 * h + 1] * f);
+    }
+    __syncthreads();
+}
+
+// Four outputs of one head, added up over the block's warps: item counts heads, and D / 4 pieces of a head.
+template <int D>
+__device__ __forceinline__ float4 block_sum(const uint8_t* smem, const float2 (*stats)[PA_HEADS], int h, int d, float& m, float& l) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][h].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; w++) {
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + (w * PA_HEADS + h) * PA_PITCH<D> + d);
+        l = fmaf(stats[w][h].y, ex2(stats[w][h].x - origin(m)), l);
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+    }
+    return o;
+}
+
+// A query row that sees nothing: zeros, and -inf.
+__device__ __forceinline__ void store_nothing(const PagedAttnArgs& a, int qrow, int head0, int heads, int D) {
+    for (int i = threadIdx.x; i < heads * D; i += blockDim.x) a.out[qrow * a.out_stride + head0 * D + i] = 0;
+    if (a.lse)
+        for (int h = threadIdx.x; h < heads; h += blockDim.x) a.lse[size_t(qrow) * a.heads + head0 + h] = -INFINITY;
+}
+
+constexpr size_t ring_bytes(int D) { return size_t(PA_WARPS) * (384 / D) * 2 * PA_TILE * D * 2; }
+
+// The line's kernel.
+template <int D, bool HALF, bool ALIGNED>
 __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, Split sp) {
     pdl_enter();
-    constexpr int ROW = D * 2, TILE_BYTES = PA_TILE * ROW, CH = D / 8, S = PA_STAGES<D>;
     extern __shared__ __align__(128) uint8_t pa_smem[];
-    // the warps' rings, afterwards the warps' outputs; then the running sums of the requests' units
-    constexpr int RING_BYTES = PA_WARPS * S * 2 * TILE_BYTES;
-    constexpr int PITCH = D + 8;  // a warp's outputs, a head a row: 8 floats further than a multiple of 32 banks
-    static_assert(PA_WARPS * PA_HEADS * PITCH * 4 <= RING_BYTES, "the outputs fit in the rings");
-    int* const upto = reinterpret_cast<int*>(pa_smem + RING_BYTES);  // [rows + 1]
+    // the warps' rings, then the running sums of the requests' places
+    int* const upto = reinterpret_cast<int*>(pa_smem + ring_bytes(D));  // [rows + 1]
     __shared__ float2 stats[PA_WARPS][PA_HEADS];
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, gq = lane >> 2, tq = lane & 3;
+    const int t = threadIdx.x;
     float* const parts = static_cast<float*>(a.workspace);
     float2* const part_stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(a.workspace) + PA_STATS_AT);
     const Line line = lay_out<PA_THREADS>(a, sp, upto);
     const int x0 = line.begin_of(blockIdx.x), x1 = line.begin_of(blockIdx.x + 1);
 
-    // requests that see nothing
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         if (upto[r + 1] != upto[r]) continue;
         const int qrow = query_row(a, r);
-        if (qrow < 0) continue;
-        for (int i = t; i < a.heads * D; i += PA_THREADS) a.out[qrow * a.out_stride + i] = 0;
-        if (a.lse)
-            for (int h = t; h < a.heads; h += PA_THREADS) a.lse[size_t(qrow) * a.heads + h] = -INFINITY;
+        if (qrow >= 0) store_nothing(a, qrow, 0, a.heads, D);
     }
 
-    const int group = a.heads / a.cache.kv_heads;
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(pa_smem)) + warp * S * 2 * TILE_BYTES;
     for (int x = x0; x < x1;) {
         const Line::Place at = line.at(x, a.rows, sp.pairs);
-        const int r = at.r, units = at.length - PA_BEGIN, place = x - at.begin;
+        const int units = at.length - PA_BEGIN, place = x - at.begin;
         const int stop = min(at.length, place + (x1 - x));
         const int u = max(place - PA_BEGIN, 0), take = stop - PA_BEGIN - u;  // its units here: [u, u + take)
         const int slot = 2 * blockIdx.x + (x != x0);
         x += stop - place;
         if (take <= 0) continue;
-        const int kv = at.pair / sp.per_kv, h0 = (at.pair % sp.per_kv) * PA_HEADS;
-        const int heads = min(PA_HEADS, group - h0), head0 = kv * group + h0;
-        const int qrow = query_row(a, r);
-        const int n = min(max(a.lens[r], 0), a.max_len), first = a.window > 0 ? max(0, n - a.window) : 0;
-        const int k0 = first + u * sp.unit, k1 = min((long long)n, k0 + (long long)take * sp.unit);
-        const bool whole = take == units;
-        const int* table = a.table + size_t(r) * a.table_stride;
-        const int tiles = (k1 - k0 + PA_TILE - 1) / PA_TILE;
-        const int mine = tiles > warp ? (tiles - warp + PA_WARPS - 1) / PA_WARPS : 0;
-        // lane j < 16 (and j + 16) looks up key j of a tile: its page, -1 outside the range
-        auto page_of = [&](int j) -> int {
-            const int key = k0 + (warp + j * PA_WARPS) * PA_TILE + (lane & 15);
-            return j < mine && key < k1 ? __ldg(table + key / a.cache.page_size) : -1;
-        };
-        auto issue = [&](int j, int page) -> uint32_t {
-            const int key = k0 + (warp + j * PA_WARPS) * PA_TILE + (lane & 15);
-            long long at = -1;
-            if (page >= 0 && page < a.cache.pages)
-                at = page * a.cache.page_stride + (key % a.cache.page_size) * a.cache.token_stride + kv * a.cache.head_stride;
-            const uint32_t mask = __ballot_sync(FULL_MASK, at >= 0) & 0xffffu;
-            const uint32_t kt = ring + (j % S) * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
+        Work w;
+        w.r = at.r;
+        w.kv = sp.per_kv == 1 ? at.pair : at.pair / sp.per_kv;
+        const int h0 = (at.pair - w.kv * sp.per_kv) * PA_HEADS;
+        w.heads = min(PA_HEADS, sp.group - h0);
+        w.head0 = w.kv * sp.group + h0;
+        w.qrow = query_row(a, at.r);
+        const Seen seen(a, at.r);
+        w.first = seen.first;
+        w.k0 = seen.origin + u * sp.unit;
+        w.k1 = int(min((long long)seen.end, w.k0 + (long long)take * sp.unit));
+        w.warp = t >> 5;
+        w.warps = PA_WARPS;
+        attend<D, HALF, ALIGNED>(a, sp, w, pa_smem, stats);
 #pragma unroll
-            for (int i = 0; i < PA_TILE * CH / 32; i++) {
-                const int row = i * (32 / CH) + lane / CH, c = lane % CH;
-                const long long off = __shfl_sync(FULL_MASK, at, row);
-                const uint32_t dst = row * ROW + ((c ^ (row & 7)) << 4);
-                copy16(kt + dst, a.cache.keys + max(off, 0ll) + c * 8, off >= 0);
-                copy16(vt + dst, a.cache.values + max(off, 0ll) + c * 8, off >= 0);
-            }
-            return mask;
-        };
-        int pages[S];  // the lookups of the next tiles to copy, the ring's first ones together
-#pragma unroll
-        for (int i = 0; i < S; i++) pages[i] = page_of(i);
-        // queries: rows gq and gq + 8 of the MMA
-        uint32_t qa[D / 16][4];
-        const uint16_t* q = a.q + qrow * a.q_stride + head0 * D;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int h = gq + (i & 1) * 8, d = kk * 16 + 2 * tq + (i >> 1) * 8;
-                qa[kk][i] = h < heads ? *reinterpret_cast<const uint32_t*>(q + h * D + d) : 0u;
-            }
-        Running<D> run;
-        run.clear();
-        // tile j is copied while tile j - (S - 1) is worked on
-        uint32_t masks[S];
-#pragma unroll
-        for (int i = 0; i < S; i++) masks[i] = 0u;
-#pragma unroll 1
-        for (int j = 0; j < mine + S - 1; j++) {
-            masks[S - 1] = j < mine ? issue(j, pages[0]) : 0u;
-            asm volatile("cp.async.commit_group;" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < S - 1; i++) pages[i] = pages[i + 1];
-            pages[S - 1] = page_of(j + S);
-            if (j >= S - 1) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-                __syncwarp();
-                const uint32_t kt = ring + ((j + 1) % S) * 2 * TILE_BYTES;
-                add_tile<D, HALF>(run, qa, kt, kt + TILE_BYTES, masks[0], a.scale_log2);
-                __syncwarp();  // the tile has been read: the next copy may overwrite it
-            }
-#pragma unroll
-            for (int i = 0; i < S - 1; i++) masks[i] = masks[i + 1];
-        }
-        // join the warps
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 1);
-            run.l[h] += __shfl_xor_sync(FULL_MASK, run.l[h], 2);
-            if (tq == 0) stats[warp][gq + 8 * h] = make_float2(run.m[h], run.l[h]);
-        }
-        __syncthreads();  // every warp is done with its ring
-        float* const mid = reinterpret_cast<float*>(pa_smem);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float m = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][gq + 8 * h].x);
-            const float f = ex2(run.m[h] - origin(m));
-#pragma unroll
-            for (int j = 0; j < D / 8; j++)
-                *reinterpret_cast<float2*>(mid + (warp * PA_HEADS + gq + 8 * h) * PITCH + j * 8 + 2 * tq) =
-                    make_float2(run.o[j][2 * h] * f, run.o[j][2 * h + 1] * f);
-        }
-        __syncthreads();
-        constexpr int ITEMS = PA_HEADS * D / 4 / PA_THREADS;
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
+        for (int i = 0; i < PA_HEADS * D / 4 / PA_THREADS; i++) {
             const int item = i * PA_THREADS + t, h = item / (D / 4), d = (item % (D / 4)) * 4;
-            if (h >= heads) break;
-            float m = -INFINITY, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < PA_WARPS; w++) m = fmaxf(m, stats[w][h].x);
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < PA_WARPS; w++) {
-                const float4 v = *reinterpret_cast<const float4*>(mid + (w * PA_HEADS + h) * PITCH + d);
-                l = fmaf(stats[w][h].y, ex2(stats[w][h].x - origin(m)), l);
-                o.x += v.x;
-                o.y += v.y;
-                o.z += v.z;
-                o.w += v.w;
-            }
-            if (whole) {
-                store_row<HALF>(a, qrow, head0 + h, D, d, o, m, l);
+            if (h >= w.heads) break;
+            float m, l;
+            const float4 o = block_sum<D>(pa_smem, stats, h, d, m, l);
+            if (take == units) {
+                store_row<HALF>(a, w.qrow, w.head0 + h, D, d, o, m, l);
             } else {
                 *reinterpret_cast<float4*>(parts + (size_t(slot) * PA_HEADS + h) * D + d) = o;
                 if (d == 0) part_stats[slot * PA_HEADS + h] = make_float2(m, l);
@@ -441,6 +578,83 @@ __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn(PagedAttnArgs a, S
         }
         __syncthreads();  // the rings and stats are free again
     }
+}
+
+// The kernel of few requests of moderate length: a cluster takes one request and head, its warps every tile in
+// turn, and the blocks' sums are joined through distributed shared memory, each block taking some heads. One
+// launch, no line to lay out and no join.
+template <int D, bool HALF, bool ALIGNED>
+__global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn_cluster(PagedAttnArgs a, Split sp) {
+    pdl_enter();
+    extern __shared__ __align__(128) uint8_t pa_smem[];
+    __shared__ float2 stats[PA_WARPS][PA_HEADS];
+    __shared__ float2 sums[PA_HEADS];
+    // the block's outputs, behind the warps'
+    constexpr int AT = PA_WARPS * PA_HEADS * PA_PITCH<D> * 4;
+    static_assert(AT + PA_HEADS * D * 4 <= int(ring_bytes(D)), "the block's outputs fit behind the warps'");
+    float* const part = reinterpret_cast<float*>(pa_smem + AT);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int t = threadIdx.x, ranks = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+    const int at = blockIdx.x / ranks;  // the request and head
+    Work w;
+    w.r = at / sp.pairs;
+    const int pair = at - w.r * sp.pairs;
+    w.kv = sp.per_kv == 1 ? pair : pair / sp.per_kv;
+    const int h0 = (pair - w.kv * sp.per_kv) * PA_HEADS;
+    w.heads = min(PA_HEADS, sp.group - h0);
+    w.head0 = w.kv * sp.group + h0;
+    w.qrow = query_row(a, w.r);
+    if (w.qrow < 0) return;  // the whole cluster
+    const Seen seen(a, w.r);
+    if (seen.end <= seen.first) {
+        if (rank == 0) store_nothing(a, w.qrow, w.head0, w.heads, D);
+        return;
+    }
+    w.first = seen.first;
+    w.k0 = seen.origin;
+    w.k1 = seen.end;
+    w.warp = rank * PA_WARPS + (t >> 5);
+    w.warps = ranks * PA_WARPS;
+    attend<D, HALF, ALIGNED>(a, sp, w, pa_smem, stats);
+#pragma unroll
+    for (int i = 0; i < PA_HEADS * D / 4 / PA_THREADS; i++) {
+        const int item = i * PA_THREADS + t, h = item / (D / 4), d = (item % (D / 4)) * 4;
+        float m, l;
+        *reinterpret_cast<float4*>(part + h * D + d) = block_sum<D>(pa_smem, stats, h, d, m, l);
+        if (d == 0) sums[h] = make_float2(m, l);
+    }
+    cluster.sync();
+    const int share = PA_HEADS / ranks;  // heads of a block
+    for (int item = t; item < share * (D / 4); item += PA_THREADS) {
+        const int h = rank * share + item / (D / 4), d = (item % (D / 4)) * 4;
+        if (h >= w.heads) break;
+        float2 st[PA_CLUSTER];
+        float4 v[PA_CLUSTER];
+#pragma unroll
+        for (int c = 0; c < PA_CLUSTER; c++) {  // all reads in flight together
+            st[c] = make_float2(-INFINITY, 0.f);
+            v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c < ranks) {
+                st[c] = cluster.map_shared_rank(sums, c)[h];
+                v[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part, c) + h * D + d);
+            }
+        }
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int c = 0; c < PA_CLUSTER; c++) m = fmaxf(m, st[c].x);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < PA_CLUSTER; c++) {
+            const float f = ex2(st[c].x - origin(m));
+            l = fmaf(st[c].y, f, l);
+            o.x = fmaf(v[c].x, f, o.x);
+            o.y = fmaf(v[c].y, f, o.y);
+            o.z = fmaf(v[c].z, f, o.z);
+            o.w = fmaf(v[c].w, f, o.w);
+        }
+        store_row<HALF>(a, w.qrow, w.head0 + h, D, d, o, m, l);
+    }
+    cluster.sync();  // no block leaves while another reads its sums
 }
 
 // Adds up the pieces of the heads of a cut request. A block takes 16 / per_head heads, per_head warps each: a
@@ -475,7 +689,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Sp
         pieces = (at.begin + at.length - 1) / line.per_block - b0 + 1;
         mine = pieces > 1 && (by_pair || int(blockIdx.x) == b0 + 1);
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.cache.kv_heads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = sp.group;
     const int kv = mine ? at.pair / sp.per_kv : 0, h0 = mine ? (at.pair % sp.per_kv) * PA_HEADS : 0;
     const int h = blockIdx.y * (WARPS / per_head) + warp / per_head, part = warp % per_head;
     const int first_slot = 2 * b0 + (mine && at.begin > b0 * line.per_block);
@@ -520,12 +734,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Sp
     if (part != 0 || !inside || lane * 4 >= D) return;
     const int d = lane * 4;
     float top = -INFINITY, sum = 0.f;
-    for (int w = warp; w < warp + per_head; w++) top = fmaxf(top, stats[w].x);
+#pragma unroll
+    for (int i = 0; i < WARPS; i++)
+        if (i < per_head) top = fmaxf(top, stats[warp + i].x);
     float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = warp; w < warp + per_head; w++) {
-        const float f = ex2(stats[w].x - origin(top));
-        const float4 v = *reinterpret_cast<const float4*>(&outs[w][d]);
-        sum = fmaf(stats[w].y, f, sum);
+#pragma unroll
+    for (int i = 0; i < WARPS; i++) {
+        if (i >= per_head) continue;
+        const float f = ex2(stats[warp + i].x - origin(top));
+        const float4 v = *reinterpret_cast<const float4*>(&outs[warp + i][d]);
+        sum = fmaf(stats[warp + i].y, f, sum);
         out.x = fmaf(v.x, f, out.x);
         out.y = fmaf(v.y, f, out.y);
         out.z = fmaf(v.z, f, out.z);
@@ -534,35 +752,70 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Sp
     store_row<HALF>(a, qrow, kv * group + h0 + h, D, d, out, top, sum);
 }
 
-constexpr size_t ring_bytes(int D) { return size_t(PA_WARPS) * (384 / D) * 2 * PA_TILE * D * 2; }
+template <int D, bool HALF, bool ALIGNED>
+cudaError_t launch_main(const PagedAttnArgs& a, const Split& sp, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_shared(k_paged_attn<D, HALF, ALIGNED>, ring_bytes(D) + (PAGED_MAX_ROWS + 1) * sizeof(int), done);
+    if (e != cudaSuccess) return e;
+    return pdl_launch(k_paged_attn<D, HALF, ALIGNED>, dim3(sp.blocks), dim3(PA_THREADS), ring_bytes(D) + (a.rows + 1) * sizeof(int), s,
+                      a, sp);
+}
+
+template <int D, bool HALF, bool ALIGNED>
+cudaError_t launch_cluster(const PagedAttnArgs& a, const Split& sp, int ranks, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_shared(k_paged_attn_cluster<D, HALF, ALIGNED>, ring_bytes(D), done);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(a.rows) * sp.pairs * ranks);
+    cfg.blockDim = dim3(PA_THREADS);
+    cfg.dynamicSmemBytes = ring_bytes(D);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, k_paged_attn_cluster<D, HALF, ALIGNED>, a, sp);
+}
 
 template <int D, bool HALF>
 cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
-    const int group = a.heads / a.cache.kv_heads;
     Split sp;
-    sp.per_kv = (group + PA_HEADS - 1) / PA_HEADS;
+    sp.group = a.heads / a.cache.kv_heads;
+    sp.per_kv = (sp.group + PA_HEADS - 1) / PA_HEADS;
     sp.pairs = a.cache.kv_heads * sp.per_kv;
-    const long long longest = a.window > 0 ? std::min(a.window, a.max_len) : a.max_len;
+    sp.page_shift = -1;
+    for (int i = 0; i < 31; i++)
+        if (a.cache.page_size == 1 << i) sp.page_shift = i;
+    // keys from the first tile on
+    const long long longest = a.window > 0 ? std::min((long long)a.window + PA_TILE - 1, (long long)a.max_len) : a.max_len;
+    const bool aligned = a.cache.page_size % PA_TILE == 0;
+    if (longest > PA_WHOLE)
+        for (int ranks = PA_CLUSTER; ranks > 1; ranks /= 2)
+            if (const long long blocks = (long long)a.rows * sp.pairs * ranks;
+                blocks <= 2 * sm_count() && longest <= (long long)ranks * (blocks >= 0.8 * sm_count() ? PA_SHARE_FULL : PA_SHARE))
+                return aligned ? launch_cluster<D, HALF, true>(a, sp, ranks, s) : launch_cluster<D, HALF, false>(a, sp, ranks, s);
     // short requests stay whole; units grow only where their number would pass 31 bits
     long long unit = longest <= PA_WHOLE ? PA_WHOLE : PA_UNIT;
     while (a.rows * ((longest + unit - 1) / unit + PA_BEGIN) * sp.pairs > INT_MAX / 2) unit *= 2;
     sp.unit = int(unit);
     const long long units = (longest + unit - 1) / unit;
     sp.blocks = int(std::min(a.rows * sp.pairs * (units > 1 ? units + PA_BEGIN : 1), 2ll * sm_count()));
-    const size_t sums = (a.rows + 1) * sizeof(int), smem = ring_bytes(D) + sums;
-    static std::atomic<uint64_t> done{0};
-    cudaError_t e = allow_shared(k_paged_attn<D, HALF>, ring_bytes(D) + (PAGED_MAX_ROWS + 1) * sizeof(int), done);
-    if (e == cudaSuccess) e = pdl_launch(k_paged_attn<D, HALF>, dim3(sp.blocks), dim3(PA_THREADS), smem, s, a, sp);
+    cudaError_t e = aligned ? launch_main<D, HALF, true>(a, sp, s) : launch_main<D, HALF, false>(a, sp, s);
     if (e != cudaSuccess || units <= 1) return e;
     const int by_pair = (long long)a.rows * sp.pairs <= sp.blocks;
     // warps a head: all 16 where few heads are to be joined, so that many pieces are added at once; fewer where
     // blocks would outnumber two an SM
-    const int cut = by_pair ? a.rows * sp.pairs : sp.blocks, heads = std::min(group, PA_HEADS);
+    const int cut = by_pair ? a.rows * sp.pairs : sp.blocks, heads = std::min(sp.group, PA_HEADS);
     int per_head = JOIN_THREADS / 32;
     while (per_head > 1 && (long long)cut * heads * per_head / (JOIN_THREADS / 32) > 2 * sm_count()) per_head /= 2;
     const int heads_a_block = JOIN_THREADS / 32 / per_head;
-    return pdl_launch(k_paged_join<D, HALF>, dim3(cut, (heads + heads_a_block - 1) / heads_a_block), dim3(JOIN_THREADS), sums, s, a,
-                      sp, by_pair, per_head);
+    return pdl_launch(k_paged_join<D, HALF>, dim3(cut, (heads + heads_a_block - 1) / heads_a_block), dim3(JOIN_THREADS),
+                      (a.rows + 1) * sizeof(int), s, a, sp, by_pair, per_head);
 }
 
 }  // namespace

@@ -59,7 +59,7 @@ def test_attention_refusals(pkg):
                 window=0, scale=0.1, out=P, out_stride=2048, lse=P, workspace=P, workspace_bytes=size)
     bad = dict(cache=[cache(rt, **c) for c in BAD_CACHES], q=[None, P + 2], q_stride=[2040, 2050], q_rows=[0, 3], heads=[0, 15, 258],
                table=[None], table_stride=[0, 7], lens=[None], rows=[0, 8193], max_len=[0, 129], window=[-1],
-               scale=[math.nan, math.inf], out=[None, P + 4], out_stride=[2040, 2052], workspace=[None, P + 8],
+               scale=[math.nan, math.inf, 0.0, -0.1], out=[None, P + 4], out_stride=[2040, 2052], workspace=[None, P + 8],
                workspace_bytes=[0, size - 1])
     for args in each(good, bad):
         refused(pkg, rt.k_paged_attention, *args.values())
