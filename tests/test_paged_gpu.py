@@ -327,6 +327,42 @@ def test_attention_many_requests(torch, pkg):
     c.check(*c.run(), rows=range(0, 8192, 13))
 
 
+@pytest.mark.parametrize("rows,top,heads,kv,page,window", [(400, 700, 16, 1, 16, 0), (300, 500, 8, 4, 24, 0), (350, 900, 4, 1, 16, 301),
+                                                           (600, 300, 2, 2, 7, 290)])
+def test_attention_many_cut_requests(torch, pkg, rows, top, heads, kv, page, window):
+    """More requests and heads than blocks, some of them cut between two."""
+    lens = np.random.default_rng(rows).integers(0, top + 1, rows)
+    lens[::17] = 0
+    lens[5] = top
+    c = Case(torch, pkg.runtime, lens.tolist(), heads, kv, 64, page, window=window)
+    out, lse = c.run()
+    c.check(out, lse, rows=list(range(0, rows, 7)) + [5])
+    assert (c.run()[0] == out).all()
+
+
+@pytest.mark.parametrize("page,window", [(24, 0), (5, 0), (48, 0), (24, 4001), (16, 4001), (16, 3000)])
+def test_attention_long_odd_pages(torch, pkg, page, window):
+    c = Case(torch, pkg.runtime, [6001, 9, 4096, 0, 7777], 16, 1, 128, page, window=window, holes=[(0, 2, -1), (2, 3, -1)])
+    c.check(*c.run())
+
+
+def test_attention_packed_rows_long(torch, pkg):
+    """As test_attention_packed_rows, where the requests are cut."""
+    c = Case(torch, pkg.runtime, [9000, 70, 12001, 40, 5000], 16, 4, 128, 16)
+    counts = [1, 0, 2, 1, 0]
+    start = np.concatenate([[0], np.cumsum(counts)])
+    q = torch.randn(int(start[-1]), 16, 128, device="cuda").bfloat16()
+    rows = [r for r in range(5) if counts[r]]
+    for r in rows:
+        q[start[r + 1] - 1] = c.q[r]
+    out, lse = c.run(q=q, row_start=ints(torch, start))
+    full_out, full_lse = np.zeros((5, 16, 128)), np.zeros((5, 16))
+    for r in rows:
+        full_out[r], full_lse[r] = out[start[r + 1] - 1], lse[start[r + 1] - 1]
+    c.check(full_out, full_lse, rows=rows)
+    assert (out[1] == 3.0).all() and (lse[1] == 3.0).all()
+
+
 def test_attention_all_requests_empty(torch, pkg):
     c = Case(torch, pkg.runtime, [0] * 40, 16, 1, 128, 16)
     out, lse = c.run()
@@ -508,6 +544,44 @@ def test_sample_settings(torch, pkg, dtype, rows, vocab, stride, offset):
                 assert kept[r] == k
 
 
+@pytest.mark.parametrize("dtype,vocab,shape", [
+    ("f32", 30011, "narrow"), ("bf16", 107520, "narrow"), ("f16", 50000, "sorted"), ("f32", 107520, "sorted"), ("bf16", 40000, "steps"),
+    ("f32", 1300001, "normal"), ("bf16", 2100000, "normal"), ("f32", 20000, "zero"), ("bf16", 9000, "zero")])
+def test_sample_unusual_distributions(torch, pkg, dtype, vocab, shape):
+    """Kept sets of thousands, values next to each other or in each other's reach, rows past shared memory."""
+    rng, rows = np.random.default_rng(vocab), 3
+    x = {"narrow": lambda: 1e-3 * rng.standard_normal((rows, vocab)) + 7.0,
+         "sorted": lambda: np.repeat(-np.arange(vocab)[None] * 1e-3, rows, 0),
+         "steps": lambda: np.floor(4.0 * rng.standard_normal((rows, vocab))),
+         "normal": lambda: 3.0 * rng.standard_normal((rows, vocab)),
+         "zero": lambda: rng.standard_normal((rows, vocab)) * 10.0 ** rng.integers(-30, 1, (rows, vocab))}[shape]()
+    for k, p, mp in ((0, 1.0, 0.0), (100, 1.0, 0.0), (300, 0.9, 0.0), (700, 1.0, 0.0), (5000, 0.5, 0.0), (0, 0.3, 0.0), (0, 0.97, 0.0),
+                     (0, 0.97, 0.3), (vocab - 1, 0.999, 0.0)):
+        u = rng.random(rows).astype(np.float32)
+        ids, lp, kept, seen = run_sample(torch, pkg.runtime, x, dtype, 0.9, k, p, mp, u)
+        for r in range(rows):
+            sample_check(seen[r], ids[r], lp[r], kept[r], 0.9, k, p, mp, u[r])
+            if p == 1.0 and k:
+                assert kept[r] == k
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_sample_extreme_temperatures(torch, pkg, dtype):
+    x = np.random.default_rng(5).standard_normal((4, 3000))
+    x[1], x[2, 7], x[3, [3, 2000]] = -np.inf, -np.inf, np.inf
+    for t in (1e-30, 1e-18, 1e18, 1e30, np.inf):
+        for k, p in ((0, 1.0), (10, 1.0), (0, 0.5)):
+            ids, lp, kept, seen = run_sample(torch, pkg.runtime, x, dtype, t, k, p, None, 0.5)
+            assert ids[1] == 0 and kept[1] == 0 and np.isneginf(lp[1])
+            assert kept[3] == (1 if p == 0.5 else 2) and ids[3] == (3 if p == 0.5 else 2000)
+            for r in (0, 2):
+                full = 3000 - (r == 2)
+                if t > 1:
+                    assert kept[r] == (10 if k else full if p == 1.0 else (full + 1) // 2)
+                else:
+                    assert kept[r] == 1 and ids[r] == seen[r].argmax() and lp[r] == 0
+
+
 def test_sample_ties_go_to_the_lowest_index(torch, pkg):
     rt = pkg.runtime
     x = np.zeros((1, 3000))
@@ -575,3 +649,55 @@ def test_sample_follows_the_distribution(torch, pkg):
     ids, _, _, _ = run_sample(torch, pkg.runtime, np.repeat(x, n, 0), "f32", None, None, None, None, (np.arange(n) + 0.5) / n)
     assert (np.diff(ids) >= 0).all()
     assert np.abs(np.bincount(ids, minlength=4) / n - np.exp(x[0])).max() <= 1.5 / n
+
+
+# ------------------------------------------------------------------------------------------ all four
+
+def test_step_in_a_cuda_graph(torch, pkg):
+    """Plan, append, attention and sampling captured as one graph give what they give one by one."""
+    rt, rng = pkg.runtime, np.random.default_rng(12)
+    lens, append, page, pages, table, free, count, tokens = make_plan(3, 20, 16, 80, 1, 2, 60)
+    rows, heads, kv, dim, vocab = 20, 16, 1, 128, 5000
+    i32 = lambda v: ints(torch, v)  # noqa: E731
+    t = dict(lens=i32(lens), append=i32(append), table=i32(table), free_list=i32(free + [0] * (pages - len(free))), count=i32([count]),
+             new=i32([0] * rows), start=i32([0] * (rows + 1)), slots=i32([0] * tokens), pos=i32([0] * tokens), counts=i32([0] * 4))
+    caches = [torch.randn(pages, page, kv, dim, device="cuda").bfloat16() for _ in range(2)]
+    cache = rt.PagedCache(caches[0].data_ptr(), caches[1].data_ptr(), 0, pages, page, kv, dim, page * dim, dim, dim)
+    qkv = torch.randn(tokens, (heads + 2 * kv) * dim, device="cuda").bfloat16()
+    norms = [torch.tensor(0.1 * rng.standard_normal(dim)).bfloat16().cuda() for _ in range(2)]
+    rope, _ = rope_bits(torch, 80 * page + 1, dim)
+    q, out = (torch.zeros(tokens, heads * dim, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    work = torch.empty(rt.paged_attention_workspace(), dtype=torch.uint8, device="cuda")
+    logits = (3 * torch.randn(rows, vocab, device="cuda")).bfloat16()
+    u, ids = torch.rand(rows, device="cuda"), i32([0] * rows)
+    temperature, top_k, top_p = torch.full((rows,), 0.8, device="cuda"), i32([40] * rows), torch.full((rows,), 0.9, device="cuda")
+
+    def step(stream):
+        rt.k_paged_plan(t["lens"].data_ptr(), t["append"].data_ptr(), rows, page, pages, t["table"].data_ptr(), 80, t["free_list"].data_ptr(),
+                        t["count"].data_ptr(), t["new"].data_ptr(), t["start"].data_ptr(), t["slots"].data_ptr(), t["pos"].data_ptr(),
+                        tokens, t["counts"].data_ptr(), stream)
+        rt.k_paged_qkv(cache, qkv.data_ptr(), qkv.shape[1], tokens, heads, norms[0].data_ptr(), norms[1].data_ptr(), 1e-6, rope.data_ptr(),
+                       rope.shape[0], t["pos"].data_ptr(), t["slots"].data_ptr(), q.data_ptr(), heads * dim, stream)
+        rt.k_paged_attention(cache, q.data_ptr(), heads * dim, tokens, heads, t["table"].data_ptr(), 80, t["new"].data_ptr(), rows,
+                             t["start"].data_ptr(), 80 * page, 0, dim ** -0.5, out.data_ptr(), heads * dim, 0, work.data_ptr(),
+                             work.numel(), stream)
+        rt.k_sample(logits.data_ptr(), 0, rows, vocab, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), 0, u.data_ptr(),
+                    ids.data_ptr(), 0, 0, stream)
+
+    torch.cuda.synchronize()
+    step(0)
+    torch.cuda.synchronize()
+    results = [t["new"], t["slots"], t["counts"], t["table"], caches[0], caches[1], q, out, ids]
+    want = [r.clone() for r in results]
+    assert int((ids > 0).sum()) and float(out.float().abs().max()) > 0
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        g.capture_begin()
+        step(s.cuda_stream)
+        g.capture_end()
+        for r in (t["new"], t["slots"], t["counts"], q, out, ids):
+            r.zero_()
+        for _ in range(3):
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(results, want))
