@@ -54,6 +54,13 @@ struct Logit<0> {  // bf16
     static constexpr int KEY_SHIFT = 16;  // bits of the fp32 key that are the same for every value
     static constexpr uint16_t NOTHING = 0xff80;
     static __device__ __forceinline__ float value(uint16_t b) { return bf2f(b); }
+    // the larger of two pairs of values (or of one), and the larger value of a pair; NaN loses
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+    static __device__ __forceinline__ float larger(uint32_t a) { return fmaxf(lo_bf(a), hi_bf(a)); }
+    static constexpr uint32_t NOTHING2 = 0xff80ff80u;
 };
 template <>
 struct Logit<1> {  // fp16
@@ -61,6 +68,15 @@ struct Logit<1> {  // fp16
     static constexpr int KEY_SHIFT = 13;
     static constexpr uint16_t NOTHING = 0xfc00;
     static __device__ __forceinline__ float value(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+    static __device__ __forceinline__ float larger(uint32_t a) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+        return fmaxf(f.x, f.y);
+    }
+    static constexpr uint32_t NOTHING2 = 0xfc00fc00u;
 };
 template <>
 struct Logit<2> {  // fp32
@@ -68,6 +84,11 @@ struct Logit<2> {  // fp32
     static constexpr int KEY_SHIFT = 0;
     static constexpr uint32_t NOTHING = 0xff800000u;
     static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+    static __device__ __forceinline__ float larger(uint32_t a) { return __uint_as_float(a); }
+    static constexpr uint32_t NOTHING2 = 0xff800000u;
 };
 
 // Order-preserving key of a logit (larger is larger, -0 equals 0).
@@ -111,6 +132,24 @@ __device__ __forceinline__ u64 fixed(float e) {
     const uint32_t b = __float_as_uint(e);
     return (u64((b & 0x7fffffu) | 0x800000u) << 17) >> (127u - (b >> 23));
 }
+
+// Sum of floor(2^40 e) over few thousand e <= 1 in two 32-bit words, without a 64-bit operation or a conversion an
+// addend: adding 2^23 towards zero leaves the whole part of 2^20 e in the low mantissa bits, and what it cut off,
+// times 2^20 the same way, the next 20 bits. The words add up the floats' bits; 2^23's own are taken out at the end.
+struct WeightSum {
+    uint32_t high = 0, low = 0, number = 0;
+    static constexpr int MOST = 4095;  // addends: 4095 * 2^20 < 2^32
+    __device__ __forceinline__ void add(float e) {
+        const float x = e * 1048576.f, whole = __fadd_rz(x, 8388608.f);
+        high += __float_as_uint(whole);
+        low += __float_as_uint(__fmaf_rz(x - (whole - 8388608.f), 1048576.f, 8388608.f));
+        number++;
+    }
+    __device__ __forceinline__ u64 total() const {
+        const uint32_t ones = number * 0x4b000000u;
+        return (u64(high - ones) << 20) + (low - ones);
+    }
+};
 
 // fraction * total / 2^24 in whole numbers (fraction <= 2^24, total < 2^62), rounded down or up
 __device__ __forceinline__ u64 share(u64 fraction, u64 total, bool up) {
@@ -554,6 +593,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     row.cached = min(cached, row.length);
     // an odd number of values a thread: neighbouring threads start in different banks
     const int per = ((row.length + SAMPLE_THREADS - 1) / SAMPLE_THREADS) | 1;
+    static_assert(SAMPLE_MAX_VOCAB / MAX_CLUSTER / SAMPLE_THREADS + 1 <= WeightSum::MOST, "a thread's weights fit their sums");
     row.mine0 = min(t * per, row.length);
     row.mine1 = min(row.mine0 + per, row.length);
 
@@ -566,8 +606,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     const u64 p24 = top_p < 1.f ? u64(rint(fmax(double(top_p), 0.0) * 16777216.0)) : 1ull << 24;
     const u64 least = max(1ull, min_p > 0.f ? u64(ceil(fmin(double(min_p), 1.0) * 1099511627776.0)) : 0ull);
 
-    // read the slice once; the largest logit (fmaxf passes over NaN)
-    float top = -INFINITY;
+    // read the slice once; the largest logit
+    uint32_t top2 = Logit<TYPE>::NOTHING2;
     constexpr int BATCH = 4;  // reads in flight together
     for (int v0 = t; v0 * VEC < row.length; v0 += BATCH * SAMPLE_THREADS) {
         uint4 x4[BATCH];
@@ -588,12 +628,12 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
         for (int b = 0; b < BATCH; b++) {
             const int j = (v0 + b * SAMPLE_THREADS) * VEC;
             if (j < row.cached) *reinterpret_cast<uint4*>(row.slice + j) = x4[b];
-            const raw* x = reinterpret_cast<const raw*>(&x4[b]);
+            const uint32_t pairs[4] = {x4[b].x, x4[b].y, x4[b].z, x4[b].w};
 #pragma unroll
-            for (int e = 0; e < VEC; e++) top = fmaxf(top, Logit<TYPE>::value(x[e]));
+            for (int e = 0; e < 4; e++) top2 = Logit<TYPE>::max2(top2, pairs[e]);
         }
     }
-    top = warp_max(top);
+    float top = warp_max(Logit<TYPE>::larger(top2));
     if ((t & 31) == 0) shared.scan[t >> 5] = __float_as_uint(top);
     __syncthreads();
     row.cluster.barrier_wait();
@@ -653,21 +693,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     if (nucleus) {
         // all weights, those near the top, and a list of the latter
         const float near = far * 0.3f;
-        u64 all_weight = 0, near_weight = 0;
+        WeightSum all_weight;
+        u64 near_weight = 0;
         row.start_list();
         auto add = [&](float x, float e, int i) {
-            if (e >= LEAST) {
-                const u64 f = fixed(e);
-                all_weight += f;
-                if (!(top - x > near)) {
-                    near_weight += f;
-                    row.add_to_list(x, i);
-                }
+            all_weight.add(e >= LEAST ? e : 0.f);
+            if (!(top - x > near) && e >= LEAST) {
+                near_weight += fixed(e);
+                row.add_to_list(x, i);
             }
         };
         if (edge) row.each([&](float x) { return x > -INFINITY && row.key(x) >= edge ? row.like(x) : 0.f; }, add);
         else row.each(row.like, add);
-        Pair sums = row.block_add({all_weight, near_weight});
+        Pair sums = row.block_add({all_weight.total(), near_weight});
         const int n = row.deliver(sums);
         const u64 cut_off = ties < at_edge ? (at_edge - ties) * row.weight(key_value<KS>(edge)) : 0ull;
         const u64 run = sums.a - cut_off, need = max(share(p24, run, true), 1ull);
@@ -710,13 +748,12 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     // w >= least, both whole, is e >= least / 2^40: exact in fp32, min_p having 24 bits
     const float least_e = float(least) * LEAST;
     const uint32_t tie_end = ties < at_edge ? uint32_t(ties) : 0xffffffffu;
-    u64 my_weight = 0;
+    WeightSum sum;
     uint32_t my_count = 0, tie = uint32_t(first_tie);
     auto add = [&](float e) {
-        if (e >= least_e) {
-            my_weight += fixed(e);
-            my_count++;
-        }
+        const bool kept = e >= least_e;
+        sum.add(kept ? e : 0.f);
+        my_count += kept;
     };
     if (edge) {
         row.each([&](float x) { return x > -INFINITY ? row.key(x) : 0u; },
@@ -726,6 +763,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     } else {
         row.each(row.like, [&](float, float e, int) { add(e); });
     }
+    const u64 my_weight = sum.total();
     Pair ahead;
     const Pair total = row.exchange(row.block_add({my_weight, my_count}), ahead);
     const u64 target = share(m, total.a, false);
