@@ -15,10 +15,10 @@
 //   k values are at least that large; for k up to twice the warps the j that leaves a quarter more than k if large
 //   values lie anywhere (n ids spread over N warps miss N e^{-n/N} of them), and k are counted. Else, and when
 //   that fails, those up to the step of a histogram where k is reached;
-// - under top-p, the values within 8.3 T of the top (there, one in 4000 as likely), listed in the pass that adds up all weights. When those do not
-//   hold p or are too many, a histogram of what could be kept at all (what V times over would fit into the part
-//   left out cannot) gives the step where p is reached. Histograms have 256 equal steps of (max - x), which spreads
-//   the many near-equal logits that bins by bits of x would pile onto a few addresses.
+// - under top-p, the values within 8.3 T of the top (there, one in 4000 as likely), beside the sum of all weights.
+//   When those do not hold p or are too many, a histogram of what could be kept at all (what V times over would fit
+//   into the part left out cannot) gives the step where p is reached. Histograms have 256 equal steps of
+//   (max - x), which spreads the many near-equal logits that bins by bits of x would pile onto a few addresses.
 // A larger superset has its threshold narrowed down by histograms over the keys inside the step, and all
 // blocks finish the row. w = 0 beyond 27.8 T. Bound by instructions (an exponential an id at least, unless top-k
 // comes first) for many rows, by the cluster barriers for one.
@@ -354,9 +354,14 @@ struct Row {
         if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
     }
-    __device__ __forceinline__ void add_to_list(float x, int i) {
-        const uint32_t n = atomicAdd(&sh.listed, 1u);
-        if (n < LIST) sh.list[n] = u64(~key(x)) << 32 | uint32_t(begin + i - lead);
+    // this block's values x >= from, down to `far` below the top
+    __device__ __forceinline__ void list_from(float from, float far) {
+        each([&](float x) { return x >= from && x > -INFINITY && !(top - x > far); },
+             [&](float x, bool wanted, int i) {
+                 if (!wanted) return;
+                 const uint32_t n = atomicAdd(&sh.listed, 1u);
+                 if (n < LIST) sh.list[n] = u64(~key(x)) << 32 | uint32_t(begin + i - lead);
+             });
     }
     // Brings the blocks' lists together in the first block; the number of ids, or -1 when they do not fit. Each block
     // leaves up to its share in the first block's inbox before the barrier that makes the numbers known; only when
@@ -397,13 +402,10 @@ struct Row {
         }
         return int(total);
     }
-    // Lists the values x >= from, down to `far` below the top.
+    // Both.
     __device__ __forceinline__ int gather(float from, float far) {
         start_list();
-        each([&](float x) { return x >= from && x > -INFINITY && !(top - x > far); },
-             [&](float x, bool wanted, int i) {
-                 if (wanted) add_to_list(x, i);
-             });
+        list_from(from, far);
         Pair none{0, 0};
         return deliver(none);
     }
@@ -691,20 +693,19 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
         }
     }
     if (nucleus) {
-        // all weights, those near the top, and a list of the latter
-        const float near = far * 0.3f;
+        // all weights; then a list of the values near the top, and what those weigh (a pass of its own: filling the
+        // list inside the first one made its loop so long that it took twice the time)
         WeightSum all_weight;
-        u64 near_weight = 0;
-        row.start_list();
-        auto add = [&](float x, float e, int i) {
-            all_weight.add(e >= LEAST ? e : 0.f);
-            if (!(top - x > near) && e >= LEAST) {
-                near_weight += fixed(e);
-                row.add_to_list(x, i);
-            }
-        };
+        auto add = [&](float, float e, int) { all_weight.add(e >= LEAST ? e : 0.f); };
         if (edge) row.each([&](float x) { return x > -INFINITY && row.key(x) >= edge ? row.like(x) : 0.f; }, add);
         else row.each(row.like, add);
+        const float near = far * 0.3f;
+        row.start_list();
+        row.list_from(edge ? key_value<KS>(edge) : -INFINITY, near);
+        __syncthreads();
+        u64 near_weight = 0;
+        for (int i = t; i < min(int(shared.listed), LIST); i += SAMPLE_THREADS)
+            near_weight += row.weight(key_value<KS>(uint32_t(~shared.list[i] >> 32)));
         Pair sums = row.block_add({all_weight.total(), near_weight});
         const int n = row.deliver(sums);
         const u64 cut_off = ties < at_edge ? (at_edge - ties) * row.weight(key_value<KS>(edge)) : 0ull;
@@ -809,10 +810,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
 template <int TYPE>
 cudaError_t launch(const SampleArgs& a, cudaStream_t s) {
     constexpr int SIZE = TYPE == 2 ? 4 : 2, VEC = 16 / SIZE;
-    // blocks a row: enough that two blocks' slices fit an SM, more while all blocks still run at once
+    // blocks a row: enough that two blocks' slices fit an SM, and more while every block still has an SM of its own (32
+    // rows of 107,520 by top-k: 13.3 us on 4 blocks a row, 18 us on 8, which share SMs)
     int ranks = 1;
-    while (ranks < MAX_CLUSTER && ((long long)a.vocab * SIZE > (long long)ranks * (SLICE_BYTES / 4 * 3) || a.rows * ranks <= 148) &&
-           a.vocab / ranks > 2048)
+    while (ranks < MAX_CLUSTER && a.vocab / ranks > 2048 &&
+           ((long long)a.vocab * SIZE > (long long)ranks * (SLICE_BYTES / 4 * 3) || a.rows * ranks <= 74))
         ranks *= 2;
     const int len = ((a.vocab + VEC - 1 + ranks - 1) / ranks + VEC - 1) / VEC * VEC;
     const int cached = std::min(len, SLICE_BYTES / SIZE);
