@@ -49,7 +49,6 @@ constexpr int PA_CLUSTER = 8;
 constexpr int PA_SHARE = 264;
 constexpr int PA_SHARE_FULL = 640;
 constexpr int PA_MAX_BLOCKS = 592;
-constexpr int JOIN_THREADS = 512;
 // tiles in a warp's ring: 96 KB a block, two blocks an SM
 template <int D>
 constexpr int PA_STAGES = 384 / D;
@@ -657,19 +656,19 @@ __global__ void __launch_bounds__(PA_THREADS, 2) k_paged_attn_cluster(PagedAttnA
     cluster.sync();  // no block leaves while another reads its sums
 }
 
-// Adds up the pieces of the heads of a cut request. A block takes 16 / per_head heads, per_head warps each: a
-// warp adds every per_head-th piece, then the warps of a head are added. Block x finds its request and head
-// on the line before it waits for the pieces: request and head x, or, when there are more of those than
-// blocks, the one that block x of k_paged_attn begins inside.
-template <int D, bool HALF>
-__global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Split sp, int by_pair, int per_head) {
-    constexpr int WARPS = JOIN_THREADS / 32, VEC = D / 32;
+// Adds up the pieces of the heads of a cut request. A block takes WARPS / PER_HEAD heads, PER_HEAD warps each: a
+// warp adds every PER_HEAD-th piece, BATCH reads in flight together, then the warps of a head are added. Block x
+// finds its request and head on the line before it waits for the pieces: request and head x, or, when there are
+// more of those than blocks, the one that block x of k_paged_attn begins inside.
+template <int D, bool HALF, int WARPS, int PER_HEAD, int BATCH>
+__global__ void __launch_bounds__(WARPS * 32) k_paged_join(PagedAttnArgs a, Split sp, int by_pair) {
+    constexpr int VEC = D / 32;
     typedef typename std::conditional<D == 128, float4, float2>::type Vec;
     extern __shared__ int join_upto[];  // [rows + 1]
     __shared__ __align__(16) float outs[WARPS][D];
     __shared__ float2 stats[WARPS];
     // The lengths may be read here: whatever wrote them ended before k_paged_attn began.
-    const Line line = lay_out<JOIN_THREADS>(a, sp, join_upto);
+    const Line line = lay_out<WARPS * 32>(a, sp, join_upto);
     Line::Place at;
     bool mine;
     if (by_pair) {
@@ -691,7 +690,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Sp
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = sp.group;
     const int kv = mine ? at.pair / sp.per_kv : 0, h0 = mine ? (at.pair % sp.per_kv) * PA_HEADS : 0;
-    const int h = blockIdx.y * (WARPS / per_head) + warp / per_head, part = warp % per_head;
+    const int h = blockIdx.y * (WARPS / PER_HEAD) + warp / PER_HEAD, part = warp % PER_HEAD;
     const int first_slot = 2 * b0 + (mine && at.begin > b0 * line.per_block);
     pdl_enter();
     if (!mine) return;
@@ -702,14 +701,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Sp
     __align__(16) float o[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) o[i] = 0.f;
-    constexpr int BATCH = 6;  // pieces whose reads are in flight together
     const bool inside = h < min(PA_HEADS, group - h0);
-    for (int p0 = inside ? part : pieces; p0 < pieces; p0 += per_head * BATCH) {
+    for (int p0 = inside ? part : pieces; p0 < pieces; p0 += PER_HEAD * BATCH) {
         float2 st[BATCH];
         __align__(16) float v[BATCH][VEC];
 #pragma unroll
         for (int b = 0; b < BATCH; b++) {
-            const int p = p0 + b * per_head, slot = p == 0 ? first_slot : 2 * (b0 + p);
+            const int p = p0 + b * PER_HEAD, slot = p == 0 ? first_slot : 2 * (b0 + p);
             st[b] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int i = 0; i < VEC; i++) v[b][i] = 0.f;
@@ -730,17 +728,16 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_paged_join(PagedAttnArgs a, Sp
     }
     *reinterpret_cast<Vec*>(&outs[warp][lane * VEC]) = *reinterpret_cast<const Vec*>(o);
     if (lane == 0) stats[warp] = make_float2(m, l);
-    __syncthreads();
+    if (PER_HEAD == 1) __syncwarp();
+    else __syncthreads();
     if (part != 0 || !inside || lane * 4 >= D) return;
     const int d = lane * 4;
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < WARPS; i++)
-        if (i < per_head) top = fmaxf(top, stats[warp + i].x);
+    for (int i = 0; i < PER_HEAD; i++) top = fmaxf(top, stats[warp + i].x);
     float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < WARPS; i++) {
-        if (i >= per_head) continue;
+    for (int i = 0; i < PER_HEAD; i++) {
         const float f = ex2(stats[warp + i].x - origin(top));
         const float4 v = *reinterpret_cast<const float4*>(&outs[warp + i][d]);
         sum = fmaf(stats[warp + i].y, f, sum);
@@ -808,14 +805,12 @@ cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
     cudaError_t e = aligned ? launch_main<D, HALF, true>(a, sp, s) : launch_main<D, HALF, false>(a, sp, s);
     if (e != cudaSuccess || units <= 1) return e;
     const int by_pair = (long long)a.rows * sp.pairs <= sp.blocks;
-    // warps a head: all 16 where few heads are to be joined, so that many pieces are added at once; fewer where
-    // blocks would outnumber two an SM
+    // 16 warps a head and 192 reads in flight where few heads have many pieces; else a warp a head
     const int cut = by_pair ? a.rows * sp.pairs : sp.blocks, heads = std::min(sp.group, PA_HEADS);
-    int per_head = JOIN_THREADS / 32;
-    while (per_head > 1 && (long long)cut * heads * per_head / (JOIN_THREADS / 32) > 2 * sm_count()) per_head /= 2;
-    const int heads_a_block = JOIN_THREADS / 32 / per_head;
-    return pdl_launch(k_paged_join<D, HALF>, dim3(cut, (heads + heads_a_block - 1) / heads_a_block), dim3(JOIN_THREADS),
-                      (a.rows + 1) * sizeof(int), s, a, sp, by_pair, per_head);
+    const size_t sums = (a.rows + 1) * sizeof(int);
+    if (cut * heads <= 2 * sm_count())
+        return pdl_launch(k_paged_join<D, HALF, 16, 16, 12>, dim3(cut, heads), dim3(512), sums, s, a, sp, by_pair);
+    return pdl_launch(k_paged_join<D, HALF, 4, 1, 4>, dim3(cut, (heads + 3) / 4), dim3(128), sums, s, a, sp, by_pair);
 }
 
 }  // namespace
