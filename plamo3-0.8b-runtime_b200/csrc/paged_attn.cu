@@ -160,10 +160,11 @@ struct Offsets {
     }
 };
 
-// Adds one tile of 16 keys (at kt, values behind them) of which those in `mask` are visible.
+// Adds one tile of 16 keys (at kt, values behind them) of which those in `mask` are visible. upper: there are more
+// than 8 heads (rows 8 to 15 of the MMA); without it their softmax is skipped.
 template <int D, bool HALF>
 __device__ __forceinline__ void add_tile(Running<D>& run, const uint32_t (&qa)[D / 16][4], const Offsets<D>& off, uint32_t kt,
-                                         uint32_t mask, float scale) {
+                                         uint32_t mask, float scale, bool upper) {
     const int tq = threadIdx.x & 3;
     // even and odd k-steps are added up apart: half the length of a chain of dependent MMAs
     float acc[2][4], odd[2][4];
@@ -193,6 +194,11 @@ __device__ __forceinline__ void add_tile(Running<D>& run, const uint32_t (&qa)[D
     float fade[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
+        if (h == 1 && !upper) {
+            fade[1] = 1.f;
+            ph[1] = ph[3] = pl[1] = pl[3] = 0u;
+            break;
+        }
         float top = fmaxf(fmaxf(acc[0][2 * h], acc[0][2 * h + 1]), fmaxf(acc[1][2 * h], acc[1][2 * h + 1]));
         top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 1));
         top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 2));
@@ -461,7 +467,7 @@ __device__ __forceinline__ void attend(const PagedAttnArgs& a, const Split& sp, 
         if (j >= S - 1) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
             __syncwarp();
-            add_tile<D, HALF>(run, qa, at, from, masks[0], a.scale_log2);
+            add_tile<D, HALF>(run, qa, at, from, masks[0], a.scale_log2, w.heads > 8);
             __syncwarp();  // the tile has been read: the next copy may overwrite it
             from = from + 2 * TILE_BYTES == ring_end ? ring : from + 2 * TILE_BYTES;
         }

@@ -11,9 +11,9 @@
 // read from global memory, and sums and histograms are exchanged through distributed shared memory, one
 // cluster barrier each. What is kept is nearly always a small head of the vocabulary, so the aim is to name a
 // superset of it of at most 1024 ids, which the first block sorts and finishes alone:
-// - under top-k, the values from the j-th largest of the warps' maxima up: for k up to half the warps j = k, as
-//   k values are at least that large; for k up to twice the warps the j that leaves a quarter more than k if large
-//   values lie anywhere (n ids spread over N warps miss N e^{-n/N} of them), and k are counted. Else, and when
+// - under top-k, the values from the j-th largest of 128 thread groups' maxima up: for k up to half the groups j = k,
+//   as k values are at least that large; for k up to twice the groups the j that leaves a quarter more than k if large
+//   values lie anywhere (n ids spread over N groups miss N e^{-n/N} of them), and k are counted. Else, and when
 //   that fails, those up to the step of a histogram where k is reached;
 // - under top-p, the values within 8.3 T of the top (there, one in 4000 as likely), beside the sum of all weights.
 //   When those do not hold p or are too many, a histogram of what could be kept at all (what V times over would fit
@@ -42,6 +42,7 @@ constexpr int BINS = 256;
 constexpr int LIST = 1024;               // ids that the first block can finish alone
 constexpr int FEW = 128;                 // ids that are compared each with each rather than sorted
 constexpr int MAX_CLUSTER = 8;
+constexpr int GROUPS = MAX_CLUSTER * SAMPLE_WARPS;  // of a cluster: a warp of 8 blocks, ... 4 lanes of one
 constexpr int SLICE_BYTES = 128 * 1024;  // most of a slice kept in shared memory; the rest is read again
 constexpr float SPAN = 27.8f;            // 2^40 exp(-27.8) < 1
 typedef unsigned long long u64;
@@ -185,12 +186,12 @@ struct Pair {
 struct Shared {
     u64 hist[2][BINS];  // two, used in turn: one may still be read by other blocks while the next fills
     Pair exchange[4][MAX_CLUSTER];  // likewise; [i][c] is written by block c
-    static_assert(LIST == 2 * SAMPLE_THREADS, "two entries a thread");
+    static_assert(LIST == 2 * SAMPLE_THREADS && GROUPS * 4 == SAMPLE_THREADS, "two entries a thread, four threads a group");
     u64 list[LIST];     // ~key << 32 | id, so ascending order is what ties need; the first block's takes in all
     u64 inbox[LIST];    // of the first block: an equal share for every block of the cluster; later a shorter list
     uint32_t listed, counts[MAX_CLUSTER];
     u64 few[FEW];       // weights of listed ids
-    float tops[MAX_CLUSTER * SAMPLE_WARPS];  // every warp's largest value
+    float tops[GROUPS];  // the largest value of every group of threads
     float least_top;
     Pair warp_pairs[SAMPLE_WARPS];
     u64 scan[SAMPLE_WARPS];
@@ -519,6 +520,7 @@ struct Row {
             return v;
         };
         uint32_t place = 0;
+#pragma unroll 8
         for (int j = part; j < n; j += team) place += list[j] < mine;
         place = uint32_t(team_add(place));
         u64 w = i < n && place < uint32_t(k) ? weight(key_value<KS>(uint32_t(~mine >> 32))) : 0ull;
@@ -527,6 +529,7 @@ struct Row {
             const u64 run = run_known ? run_known : block_add({part == 0 ? w : 0ull, 0}).a, need = max(share(p24, run, true), 1ull);
             __syncthreads();
             u64 before = 0;
+#pragma unroll 8
             for (int j = part; j < n; j += team) before += list[j] < mine ? sh.few[j] : 0ull;
             if (team_add(before) >= need) w = 0;
             __syncthreads();
@@ -536,6 +539,7 @@ struct Row {
         const Pair total = block_add({part == 0 ? w : 0ull, part == 0 && w});
         const u64 target = share(m, total.a, false);
         u64 upto = 0;  // kept weight of the lower ids
+#pragma unroll 8
         for (int j = part; j < n; j += team) upto += uint32_t(list[j]) < uint32_t(mine) ? sh.few[j] : 0ull;
         upto = team_add(upto);
         if (part == 0 && upto <= target && target < upto + w) {
@@ -635,16 +639,15 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
             for (int e = 0; e < 4; e++) top2 = Logit<TYPE>::max2(top2, pairs[e]);
         }
     }
-    float top = warp_max(Logit<TYPE>::larger(top2));
-    if ((t & 31) == 0) shared.scan[t >> 5] = __float_as_uint(top);
-    __syncthreads();
+    const int lanes = 4 * row.ranks;  // of a group
+    float top = Logit<TYPE>::larger(top2);
+    for (int o = 1; o < lanes; o *= 2) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
     row.cluster.barrier_wait();
-    const int warps = row.ranks * SAMPLE_WARPS;
-    if (t < warps)
-        row.cluster.map_shared_rank(shared.tops, t / SAMPLE_WARPS)[row.rank * SAMPLE_WARPS + t % SAMPLE_WARPS] =
-            __uint_as_float(uint32_t(shared.scan[t % SAMPLE_WARPS]));
+    // every group's largest value to every block: lane c of a group (it has at least as many) writes to block c
+    if (t % lanes < row.ranks)
+        row.cluster.map_shared_rank(shared.tops, t % lanes)[(row.rank * SAMPLE_THREADS + t) / lanes] = top;
     row.cluster.sync();
-    for (int i = t & 31; i < warps; i += 32) top = fmaxf(top, shared.tops[i]);
+    for (int i = t & 31; i < GROUPS; i += 32) top = fmaxf(top, shared.tops[i]);
     top = warp_max(top);
     row.top = top;
     row.like.set(top, T);
@@ -655,21 +658,29 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
     typedef typename Row<TYPE>::Steps Steps;
     constexpr int KS = Logit<TYPE>::KEY_SHIFT;
 
+    if (k < V && V <= LIST) {  // all of them
+        const int n = row.gather(-INFINITY, far);
+        if (n > 0) {
+            row.finish_list(a, r, n, k, p24, least, m, 0);
+            return;
+        }
+    }
     // kept: keys above `edge`, and the first `ties` (in index order) of the `at_edge` values at it
     uint32_t edge = 0;
     u64 ties = 0, at_edge = 0, before, amount;
-    if (k <= 2 * warps) {
-        const int j = k <= warps / 2 ? k : min(warps, int(ceilf(warps * (1.f - __expf(-(1.25f * k + 24.f) / warps)))));
-        // the j-th largest of the warps' maxima: a quarter of them for each of four threads to compare with
+    if (k <= 2 * GROUPS) {
+        const int some = __syncthreads_count(t < GROUPS && shared.tops[t % GROUPS] > -INFINITY);  // groups that have a value
+        const int wanted = k <= GROUPS / 2 ? k : int(ceilf(GROUPS * (1.f - __expf(-(1.25f * k + 24.f) / GROUPS))));
+        const int j = max(min(wanted, some), 1);
+        // the j-th largest of the groups' maxima: a quarter of them for each of four threads to compare with
         const int i = t / 4;
         int above = 0;
-        if (i < warps)
 #pragma unroll 8
-            for (int o = t & 3; o < warps; o += 4)
-                above += shared.tops[o] > shared.tops[i] || (shared.tops[o] == shared.tops[i] && o < i);
+        for (int o = t & 3; o < GROUPS; o += 4)
+            above += shared.tops[o] > shared.tops[i] || (shared.tops[o] == shared.tops[i] && o < i);
         above += __shfl_xor_sync(FULL_MASK, above, 1);
         above += __shfl_xor_sync(FULL_MASK, above, 2);
-        if (i < warps && above == j - 1) shared.least_top = shared.tops[i];
+        if (above == j - 1) shared.least_top = shared.tops[i];
         __syncthreads();
         const float from = shared.least_top;
         const int n = row.gather(from, far);
