@@ -161,7 +161,8 @@ PLAMO_API int plamo_k_paged_plan(const int32_t* lens, const int32_t* append, int
  * and are rotated (rotate-half) by the row of rope [rope_rows][head_dim / 2] at the token's position (u32 =
  * bf16 cos bits | sin bits << 16; NULL: no rotation, positions unused). Queries go to q (q_stride elements
  * apart), keys and values to the cache's slot slots[t]. A token whose slot is outside the cache or whose
- * position is outside rope is not appended and its query row is zero. Two tokens must not share a slot.
+ * position is outside rope is not appended and its query row is zero. Two tokens must not share a slot; q and
+ * the cache must not overlap qkv.
  * Pointers 16-byte aligned, strides multiples of 8. */
 PLAMO_API int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv, int64_t qkv_stride, int tokens, int heads,
                                 const void* q_norm, const void* k_norm, float eps, const uint32_t* rope, int rope_rows,

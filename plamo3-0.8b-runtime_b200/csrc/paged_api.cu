@@ -4,6 +4,7 @@
 
 #include <climits>
 #include <cmath>
+#include <cstdio>
 #include <string>
 
 namespace plamo {
@@ -13,15 +14,15 @@ using namespace plamo;
 
 namespace {
 
-int invalid(const char* what) {
-    g_error = what;
+// Nothing may be thrown through the C entry points: without memory for its words a failure stays a status.
+int invalid(const char* what, const char* more = "") {
+    try {
+        g_error = std::string(what) + more;
+    } catch (...) {
+    }
     return 1;
 }
-int launched(cudaError_t e) {
-    if (e == cudaSuccess) return 0;
-    g_error = std::string("CUDA error: ") + cudaGetErrorString(e);
-    return 1;
-}
+int launched(cudaError_t e) { return e == cudaSuccess ? 0 : invalid("CUDA error: ", cudaGetErrorString(e)); }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Null, or the words that say what is wrong with a cache descriptor.
@@ -94,9 +95,10 @@ int plamo_k_paged_attention(const plamo_paged_cache* cache, const void* q, int64
         return invalid("Invalid paged attention arguments");
     if (!aligned16(q) || !aligned16(out)) return invalid("Paged attention pointers must be 16-byte aligned");
     if (!workspace || !aligned16(workspace) || workspace_bytes < paged_attention_workspace()) {
-        g_error = "Paged attention workspace too small or not 16-byte aligned: " +
-                  std::to_string(paged_attention_workspace()) + " bytes needed";
-        return 1;
+        char words[96];
+        std::snprintf(words, sizeof words, "Paged attention workspace too small or not 16-byte aligned: %zu bytes needed",
+                      paged_attention_workspace());
+        return invalid(words);
     }
     PagedAttnArgs a{cache_args(cache), static_cast<const uint16_t*>(q), q_stride, q_rows, heads, table, table_stride, lens,
                     rows, row_start, max_len, window, float(double(scale) * 1.4426950408889634), static_cast<uint16_t*>(out),

@@ -268,12 +268,16 @@ struct Split {
     int blocks;     // of k_paged_attn
 };
 
+// A value of the lengths or row starts, from L2: k_paged_join reads them before it waits, when nothing has yet made
+// older lines of its L1 invalid.
+__device__ __forceinline__ int fresh(const int* p) { return __ldcg(p); }
+
 // The query row of request r, -1 when it has none.
 __device__ __forceinline__ int query_row(const PagedAttnArgs& a, int r) {
     int q = r;
     if (a.row_start) {
-        q = a.row_start[r + 1] - 1;
-        if (q < a.row_start[r]) return -1;
+        q = fresh(a.row_start + r + 1) - 1;
+        if (q < fresh(a.row_start + r)) return -1;
     }
     return q >= 0 && q < a.q_rows ? q : -1;
 }
@@ -309,7 +313,7 @@ struct Line {
 struct Seen {
     int first, end, origin;
     __device__ __forceinline__ Seen(const PagedAttnArgs& a, int r) {
-        end = min(max(a.lens[r], 0), a.max_len);
+        end = min(max(fresh(a.lens + r), 0), a.max_len);
         first = a.window > 0 ? max(0, end - a.window) : 0;
         origin = first & ~(PA_TILE - 1);
     }
@@ -673,7 +677,8 @@ __global__ void __launch_bounds__(WARPS * 32) k_paged_join(PagedAttnArgs a, Spli
     extern __shared__ int join_upto[];  // [rows + 1]
     __shared__ __align__(16) float outs[WARPS][D];
     __shared__ float2 stats[WARPS];
-    // The lengths may be read here: whatever wrote them ended before k_paged_attn began.
+    // The lengths may be read here: k_paged_attn let this kernel begin after its own wait, so whatever wrote them has
+    // ended and left them in L2.
     const Line line = lay_out<WARPS * 32>(a, sp, join_upto);
     Line::Place at;
     bool mine;

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(THREADS) k_paged_plan(PagedPlanArgs a) {
     __shared__ long long page_sums[THREADS / 32];
     __shared__ int granted_total, refused_total;
     const int t = threadIdx.x, P = a.page_size, width = a.table_stride;
-    const long long most = (long long)width * P;  // tokens that a table row can hold
+    const long long most = min((long long)width * P, (long long)INT_MAX);  // tokens that a table row can hold
     const int per = (a.rows + THREADS - 1) / THREADS;
     const int r0 = min(t * per, a.rows), r1 = min(r0 + per, a.rows);
     const int count0 = min(max(*a.free_count, 0), a.pages);
