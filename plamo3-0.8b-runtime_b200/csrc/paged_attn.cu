@@ -45,10 +45,10 @@ constexpr int PA_WHOLE = 256;
 constexpr int PA_BEGIN = 3;
 // A cluster of up to 8 blocks takes a request and head, of the largest size that all of them run at once at, where a
 // block's share of the longest request is at most this many keys: the first number always, the second when the
-// blocks fill most SMs. Cluster and line, us: 64 x 512 keys 7.2 and 10.7, 148 x 500 12.4 and 16.9, 32 x 2048 11.2
-// and 15.3, 48 x 2048 14.6 and 17.5. Past the second number even lengths still gain (40 x 3000 to 4000: 18.6 and
-// 21.7) but ragged ones lose, as the longest request holds up its cluster alone (74 x 100 to 2000: 14.9 and 12.8;
-// 18 x 100 to 2000, 4 KV heads: 13.7 and 12.1).
+// blocks fill most SMs. Cluster and line, us: 64 x 512 keys 7.2 and 10.7, 148 x 500 12.4 and 16.9, 32 x 2048 11.0
+// and 13.7, 48 x 2048 14.5 and 16.5. Past the second number even lengths still gain (40 x 3000 to 4000: 18.4 and
+// 20.5) but ragged ones lose, as the longest request holds up its cluster alone (74 x 100 to 2000: 14.8 and 12.7;
+// 18 x 100 to 2000, 4 KV heads: 13.7 and 11.3).
 constexpr int PA_CLUSTER = 8;
 constexpr int PA_SHARE = 264;
 constexpr int PA_SHARE_FULL = 640;
@@ -862,11 +862,13 @@ cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
     sp.join = units <= 1 ? 0 : pairs <= sp.blocks ? 1 : 2;
     cudaError_t e = aligned ? launch_main<D, HALF, true>(a, sp, s) : launch_main<D, HALF, false>(a, sp, s);
     if (e != cudaSuccess || !sp.join) return e;
-    // 16 warps a head and 128 pieces in flight where few heads have many pieces, else a warp a head: 12 x 9000 keys
-    // 19.0 us and with a warp a head 21.6
+    // More warps a head where a head has more pieces (about blocks / pairs). The call in us with 16, 8, 4 and 1 warps a
+    // head: 6 x 20000 keys, 49 pieces: 18.6, 19.3; 12 x 9000, 25 pieces: 18.1, 16.3, 17.0, 19.0; 40 x 100 to 4000, 7
+    // pieces: 15.2, 11.8, 11.0, 12.6; 74 x 100 to 2000, 4 pieces: 19.7, 13.9, 13.1, 12.5.
     const int records = sp.join == 1 ? pairs : sp.blocks, heads = std::min(sp.group, PA_HEADS);
-    if (records * heads <= 2 * sm_count())
-        return pdl_launch(k_paged_join<D, HALF, 16, 16>, dim3(records, heads), dim3(512), 0, s, a);
+    if (sp.blocks > 40 * pairs) return pdl_launch(k_paged_join<D, HALF, 16, 16>, dim3(records, heads), dim3(512), 0, s, a);
+    if (sp.blocks > 15 * pairs) return pdl_launch(k_paged_join<D, HALF, 8, 8>, dim3(records, heads), dim3(256), 0, s, a);
+    if (sp.blocks > 5 * pairs) return pdl_launch(k_paged_join<D, HALF, 8, 4>, dim3(records, (heads + 1) / 2), dim3(256), 0, s, a);
     return pdl_launch(k_paged_join<D, HALF, 4, 1>, dim3(records, (heads + 3) / 4), dim3(128), 0, s, a);
 }
 
