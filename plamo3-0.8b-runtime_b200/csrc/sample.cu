@@ -190,6 +190,9 @@ struct Shared {
     u64 list[LIST];     // ~key << 32 | id, so ascending order is what ties need; the first block's takes in all
     u64 inbox[LIST];    // of the first block: an equal share for every block of the cluster; later a shorter list
     uint32_t listed, counts[MAX_CLUSTER];
+    uint32_t found;       // 16-byte packs of the slice that hold something for the list, and which
+    uint16_t packs[LIST];
+    static_assert(SLICE_BYTES / 16 <= 65536, "a pack's number fits 16 bits");
     u64 few[FEW];       // weights of listed ids
     float tops[GROUPS];  // the largest value of every group of threads
     float least_top;
@@ -351,18 +354,33 @@ struct Row {
         }
     };
 
-    __device__ __forceinline__ void start_list() {
-        if (threadIdx.x == 0) sh.listed = 0;
-        __syncthreads();
-    }
-    // this block's values x >= from, down to `far` below the top
+    // Lists this block's values x >= from, down to `far` below the top. Few are: packs of 16 bytes are looked through
+    // by their largest value first, and the found packs then value by value (32 rows of 107,520 by top-k 12.0 us, by top-p
+    // 22.4; value by value from the start 13.7 and 24.2).
     __device__ __forceinline__ void list_from(float from, float far) {
-        each([&](float x) { return x >= from && x > -INFINITY && !(top - x > far); },
-             [&](float x, bool wanted, int i) {
-                 if (!wanted) return;
-                 const uint32_t n = atomicAdd(&sh.listed, 1u);
-                 if (n < LIST) sh.list[n] = u64(~key(x)) << 32 | uint32_t(begin + i - lead);
-             });
+        if (threadIdx.x == 0) sh.listed = sh.found = 0;
+        __syncthreads();
+        auto wanted = [&](float x) { return x >= from && x > -INFINITY && !(top - x > far); };
+        auto put_in = [&](float x, int i) {
+            const uint32_t n = atomicAdd(&sh.listed, 1u);
+            if (n < LIST) sh.list[n] = u64(~key(x)) << 32 | uint32_t(begin + i - lead);
+        };
+        const int packs = (cached + VEC - 1) / VEC;  // the last one is filled up with NOTHING
+        for (int p = threadIdx.x; p < packs; p += SAMPLE_THREADS) {
+            const uint4 v = reinterpret_cast<const uint4*>(slice)[p];
+            if (!wanted(Logit<TYPE>::larger(Logit<TYPE>::max2(Logit<TYPE>::max2(v.x, v.y), Logit<TYPE>::max2(v.z, v.w))))) continue;
+            const uint32_t n = atomicAdd(&sh.found, 1u);
+            if (n < LIST) sh.packs[n] = uint16_t(p);
+            else atomicMax(&sh.listed, LIST + 1u);  // each holds one for the list at least: too many
+        }
+        for (int i = cached + threadIdx.x; i < length; i += SAMPLE_THREADS)
+            if (const float x = at(i); wanted(x)) put_in(x, i);
+        __syncthreads();
+        const int values = int(min(sh.found, uint32_t(LIST))) * VEC;
+        for (int j = threadIdx.x; j < values; j += SAMPLE_THREADS) {
+            const int i = sh.packs[j / VEC] * VEC + j % VEC;
+            if (const float x = Logit<TYPE>::value(slice[i]); wanted(x)) put_in(x, i);
+        }
     }
     // Brings the blocks' lists together in the first block; the number of ids, or -1 when they do not fit. Each block
     // leaves up to its share in the first block's inbox before the barrier that makes the numbers known; only when
@@ -405,7 +423,6 @@ struct Row {
     }
     // Both.
     __device__ __forceinline__ int gather(float from, float far) {
-        start_list();
         list_from(from, far);
         Pair none{0, 0};
         return deliver(none);
@@ -711,7 +728,6 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
         if (edge) row.each([&](float x) { return x > -INFINITY && row.key(x) >= edge ? row.like(x) : 0.f; }, add);
         else row.each(row.like, add);
         const float near = far * 0.3f;
-        row.start_list();
         row.list_from(edge ? key_value<KS>(edge) : -INFINITY, near);
         __syncthreads();
         u64 near_weight = 0;
