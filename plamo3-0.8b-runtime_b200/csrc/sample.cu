@@ -163,10 +163,13 @@ __device__ __forceinline__ float log_share(u64 w, u64 total) {
     return logf(__fdiv_rn(float(w), float(total)));
 }
 
+// In three parts whose sums over 32 lanes fit 32 bits (the upper one's wraps as the whole sum would): three
+// independent reductions instead of five dependent exchanges of two words (0.3 to 0.5 us a call).
 __device__ __forceinline__ u64 warp_add(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
-    return v;
+    const uint32_t low = __reduce_add_sync(FULL_MASK, uint32_t(v) & 0x7ffffffu);
+    const uint32_t mid = __reduce_add_sync(FULL_MASK, uint32_t(v >> 27) & 0x7ffffffu);
+    const uint32_t high = __reduce_add_sync(FULL_MASK, uint32_t(v >> 54));
+    return (u64(high) << 54) + (u64(mid) << 27) + low;
 }
 
 // inclusive, in lane order
@@ -355,8 +358,8 @@ struct Row {
     };
 
     // Lists this block's values x >= from, down to `far` below the top. Few are: packs of 16 bytes are looked through
-    // by their largest value first, and the found packs then value by value (32 rows of 107,520 by top-k 12.0 us, by top-p
-    // 22.4; value by value from the start 13.7 and 24.2).
+    // by their largest value first, and the found packs then value by value (32 rows of 107,520 by top-k 11.6 us, by top-p
+    // 21.8; value by value from the start 1.8 more).
     __device__ __forceinline__ void list_from(float from, float far) {
         if (threadIdx.x == 0) sh.listed = sh.found = 0;
         __syncthreads();
@@ -532,14 +535,14 @@ struct Row {
                                                u64 run_known) {
         const int team = n <= FEW / 2 ? 8 : 4, i = threadIdx.x / team, part = threadIdx.x % team;
         const u64 mine = i < n ? list[i] : ~0ull;
-        auto team_add = [&](u64 v) {
+        auto team_add = [&](auto v) {
             for (int o = 1; o < team; o *= 2) v += __shfl_xor_sync(FULL_MASK, v, o);
             return v;
         };
         uint32_t place = 0;
 #pragma unroll 8
         for (int j = part; j < n; j += team) place += list[j] < mine;
-        place = uint32_t(team_add(place));
+        place = team_add(place);
         u64 w = i < n && place < uint32_t(k) ? weight(key_value<KS>(uint32_t(~mine >> 32))) : 0ull;
         if (p24 < (1ull << 24)) {
             if (part == 0 && i < FEW) sh.few[i] = w;
@@ -838,7 +841,7 @@ template <int TYPE>
 cudaError_t launch(const SampleArgs& a, cudaStream_t s) {
     constexpr int SIZE = TYPE == 2 ? 4 : 2, VEC = 16 / SIZE;
     // blocks a row: enough that two blocks' slices fit an SM, and more while every block still has an SM of its own (32
-    // rows of 107,520 by top-k: 13.3 us on 4 blocks a row, 18 us on 8, which share SMs)
+    // rows of 107,520 by top-k: 11.6 us on 4 blocks a row, 16.9 us on 8, which share SMs)
     int ranks = 1;
     while (ranks < MAX_CLUSTER && a.vocab / ranks > 2048 &&
            ((long long)a.vocab * SIZE > (long long)ranks * (SLICE_BYTES / 4 * 3) || a.rows * ranks <= 74))
