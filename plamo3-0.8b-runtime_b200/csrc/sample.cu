@@ -117,9 +117,14 @@ struct Likelihood {
         inv = __frcp_rn(T_);
         plain = !(T_ > 1e-15f && T_ < 1e15f) || top_ == INFINITY;
     }
-    __device__ __forceinline__ float operator()(float x) const {
+    // Loops over many values choose between the two outside: a branch a value keeps values from overlapping
+    // (32 rows of 107,520 unfiltered: 14.3 us, so 12.7).
+    __device__ __forceinline__ float operator()(float x) const { return plain ? slow(x) : quick(x); }
+    __device__ __forceinline__ float slow(float x) const {
+        return x == top && x > -INFINITY ? 1.f : expf(__fdiv_rn(x - top, T));
+    }
+    __device__ __forceinline__ float quick(float x) const {
         const float d = x - top;
-        if (plain) return x == top && x > -INFINITY ? 1.f : expf(__fdiv_rn(d, T));
         float q = d * inv;
         q = fmaf(fmaf(-q, T, d), inv, q);
         q = fmaf(fmaf(-q, T, d), inv, q);
@@ -249,6 +254,22 @@ struct Row {
             const float x = at(i);
             act(x, pure(x), i);
         }
+    }
+    // act(pure(x)) for all of the block's values in no order, a pack of 16 bytes at a time (32 rows by top-p: 20.0 us,
+    // value by value 20.5).
+    template <typename F, typename G>
+    __device__ __forceinline__ void each_pack(F pure, G act) const {
+        const int packs = (cached + VEC - 1) / VEC;
+        for (int p = threadIdx.x; p < packs; p += SAMPLE_THREADS) {
+            __align__(16) raw x[VEC];
+            *reinterpret_cast<uint4*>(x) = reinterpret_cast<const uint4*>(slice)[p];
+            decltype(pure(0.f)) y[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; e++) y[e] = pure(Logit<TYPE>::value(x[e]));
+#pragma unroll
+            for (int e = 0; e < VEC; e++) act(y[e]);
+        }
+        for (int i = cached + threadIdx.x; i < length; i += SAMPLE_THREADS) act(pure(at(i)));
     }
     static __device__ __forceinline__ uint32_t key(float x) { return order_key(x) >> Logit<TYPE>::KEY_SHIFT; }
 
@@ -727,9 +748,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
         // all weights; then a list of the values near the top, and what those weigh (a pass of its own: filling the
         // list inside the first one made its loop so long that it took twice the time)
         WeightSum all_weight;
-        auto add = [&](float, float e, int) { all_weight.add(e >= LEAST ? e : 0.f); };
-        if (edge) row.each([&](float x) { return x > -INFINITY && row.key(x) >= edge ? row.like(x) : 0.f; }, add);
-        else row.each(row.like, add);
+        auto add = [&](float e) { all_weight.add(e >= LEAST ? e : 0.f); };
+        if (edge) row.each_pack([&](float x) { return x > -INFINITY && row.key(x) >= edge ? row.like(x) : 0.f; }, add);
+        else if (row.like.plain) row.each_pack([&](float x) { return row.like.slow(x); }, add);
+        else row.each_pack([&](float x) { return row.like.quick(x); }, add);
         const float near = far * 0.3f;
         row.list_from(edge ? key_value<KS>(edge) : -INFINITY, near);
         __syncthreads();
@@ -792,7 +814,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
                      if (key > edge || (key == edge && tie++ < tie_end)) add(row.like(x));
                  });
     } else {
-        row.each(row.like, [&](float, float e, int) { add(e); });
+        auto put = [&](float, float e, int) { add(e); };
+        if (row.like.plain) row.each([&](float x) { return row.like.slow(x); }, put);
+        else row.each([&](float x) { return row.like.quick(x); }, put);
     }
     const u64 my_weight = sum.total();
     Pair ahead;
