@@ -118,7 +118,7 @@ struct Likelihood {
         plain = !(T_ > 1e-15f && T_ < 1e15f) || top_ == INFINITY;
     }
     // Loops over many values choose between the two outside: a branch a value keeps values from overlapping
-    // (32 rows of 107,520 unfiltered: 14.3 us, so 12.7).
+    // (32 rows of 107,520 unfiltered: 14.3 us, so 12.6).
     __device__ __forceinline__ float operator()(float x) const { return plain ? slow(x) : quick(x); }
     __device__ __forceinline__ float slow(float x) const {
         return x == top && x > -INFINITY ? 1.f : expf(__fdiv_rn(x - top, T));
@@ -201,7 +201,8 @@ struct Shared {
     uint32_t found;       // 16-byte packs of the slice that hold something for the list, and which
     uint16_t packs[LIST];
     static_assert(SLICE_BYTES / 16 <= 65536, "a pack's number fits 16 bits");
-    u64 few[FEW];       // weights of listed ids
+    u64 few[FEW], sorted[FEW];  // weights of listed ids, as listed and from the largest down
+    static_assert(FEW == 4 * 32, "four a lane");
     float tops[GROUPS];  // the largest value of every group of threads
     float least_top;
     Pair warp_pairs[SAMPLE_WARPS];
@@ -255,8 +256,8 @@ struct Row {
             act(x, pure(x), i);
         }
     }
-    // act(pure(x)) for all of the block's values in no order, a pack of 16 bytes at a time (32 rows by top-p: 20.0 us,
-    // value by value 20.5).
+    // act(pure(x)) for all of the block's values in no order, a pack of 16 bytes at a time (32 rows by top-p: 18.9 us,
+    // value by value 0.5 more).
     template <typename F, typename G>
     __device__ __forceinline__ void each_pack(F pure, G act) const {
         const int packs = (cached + VEC - 1) / VEC;
@@ -379,8 +380,8 @@ struct Row {
     };
 
     // Lists this block's values x >= from, down to `far` below the top. Few are: packs of 16 bytes are looked through
-    // by their largest value first, and the found packs then value by value (32 rows of 107,520 by top-k 11.6 us, by top-p
-    // 21.8; value by value from the start 1.8 more).
+    // by their largest value first, and the found packs then value by value (32 rows of 107,520 by top-k 11.0 us, by top-p
+    // 18.9; value by value from the start 1.8 more).
     __device__ __forceinline__ void list_from(float from, float far) {
         if (threadIdx.x == 0) sh.listed = sh.found = 0;
         __syncthreads();
@@ -419,12 +420,17 @@ struct Row {
         if (threadIdx.x < ranks) *cluster.map_shared_rank(sh.counts + rank, threadIdx.x) = mine;
         Pair unused;
         sums = exchange(sums, unused);
-        uint32_t total = 0, before = 0;
+        // thread t takes what block t / TEAM has brought, all blocks' together
+        constexpr int TEAM = SAMPLE_THREADS / MAX_CLUSTER;
+        const int giver = threadIdx.x / TEAM;
+        uint32_t total = 0, before = 0, at = 0;
         bool over = false;
-        for (int c = 0; c < ranks; c++) {
-            const uint32_t n = sh.counts[c];
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; c++) {
+            const uint32_t n = c < ranks ? sh.counts[c] : 0u;
             over |= n > share;
             before += c < rank ? n : 0u;
+            at += c < giver ? n : 0u;
             total += n;
         }
         if (total > LIST) return -1;
@@ -435,12 +441,8 @@ struct Row {
             }
             cluster.sync();
         } else if (rank == 0) {
-            uint32_t at = mine;
-            for (int c = 1; c < ranks; c++) {
-                const uint32_t n = sh.counts[c];
-                if (threadIdx.x < n) sh.list[at + threadIdx.x] = sh.inbox[c * share + threadIdx.x];  // n <= share <= 512
-                at += n;
-            }
+            if (giver > 0 && giver < ranks)
+                for (uint32_t i = threadIdx.x % TEAM; i < sh.counts[giver]; i += TEAM) sh.list[at + i] = sh.inbox[giver * share + i];
             __syncthreads();
         }
         return int(total);
@@ -483,11 +485,16 @@ struct Row {
             for (int i = threadIdx.x; i < n; i += SAMPLE_THREADS) {
                 const float x = key_value<KS>(uint32_t(~list[i] >> 32));
                 const u64 w = k < n ? 1ull : weight(x);
-                if (w) put<true>(steps(x), w);
+                if (!w) continue;
+                // 20 bits each: at most 1024 ids, so neither sum leaves 32 bits
+                uint32_t* const bin = reinterpret_cast<uint32_t*>(sh.hist[hist_turn & 1] + steps(x));
+                atomicAdd(bin, uint32_t(w) & 0xfffffu);
+                if (w >> 20) atomicAdd(bin + 1, uint32_t(w >> 20));
             }
             __syncthreads();
             const u64 need = k < n ? u64(k) : max(share(p24, run_known, true), 1ull);
-            const u64 sum = threadIdx.x < BINS ? sh.hist[hist_turn & 1][threadIdx.x] : 0ull, before = block_scan(sum);
+            const uint32_t* const bin = reinterpret_cast<const uint32_t*>(sh.hist[hist_turn & 1] + threadIdx.x % BINS);
+            const u64 sum = threadIdx.x < BINS ? (u64(bin[1]) << 20) + bin[0] : 0ull, before = block_scan(sum);
             if (before < need && need <= before + sum) sh.bin = threadIdx.x;
             __syncthreads();
             for (int i = threadIdx.x; i < n; i += SAMPLE_THREADS) {
@@ -551,7 +558,8 @@ struct Row {
         if (t == 0 && a.kept) a.kept[r] = kept;
     }
     // Places and running weights of at most FEW ids by comparing each with each, four threads (or eight) an id: fewer
-    // dependent steps than a sort.
+    // dependent steps than a sort. What top-p leaves is found by each warp for itself, from all weights in order (with
+    // sums over the block instead, 1 to 2 us more).
     __device__ __forceinline__ void finish_few(const u64* list, const SampleArgs& a, int r, int n, int k, u64 p24, u64 least, u64 m,
                                                u64 run_known) {
         const int team = n <= FEW / 2 ? 8 : 4, i = threadIdx.x / team, part = threadIdx.x % team;
@@ -565,19 +573,39 @@ struct Row {
         for (int j = part; j < n; j += team) place += list[j] < mine;
         place = team_add(place);
         u64 w = i < n && place < uint32_t(k) ? weight(key_value<KS>(uint32_t(~mine >> 32))) : 0ull;
+        if (part == 0 && i < n) sh.sorted[place] = w;
+        __syncthreads();
+        // every warp by itself: the weights in order, four a lane, and what top-p and min-p leave of them
+        const int lane = threadIdx.x & 31;
+        u64 x[4], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += x[e] = 4 * lane + e < n ? sh.sorted[4 * lane + e] : 0ull;
         if (p24 < (1ull << 24)) {
-            if (part == 0 && i < FEW) sh.few[i] = w;
-            const u64 run = run_known ? run_known : block_add({part == 0 ? w : 0ull, 0}).a, need = max(share(p24, run, true), 1ull);
-            __syncthreads();
-            u64 before = 0;
-#pragma unroll 8
-            for (int j = part; j < n; j += team) before += list[j] < mine ? sh.few[j] : 0ull;
-            if (team_add(before) >= need) w = 0;
-            __syncthreads();
+            const u64 upto = warp_scan(sum), run = run_known ? run_known : __shfl_sync(FULL_MASK, upto, 31);
+            const u64 need = max(share(p24, run, true), 1ull);
+            u64 before = upto - sum;
+            uint32_t within = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u64 y = x[e];
+                if (before < need) within++;
+                else x[e] = 0;
+                before += y;
+            }
+            if (place >= __reduce_add_sync(FULL_MASK, within)) w = 0;
         }
         if (w < least) w = 0;
         if (part == 0 && i < FEW) sh.few[i] = w;
-        const Pair total = block_add({part == 0 ? w : 0ull, part == 0 && w});
+        sum = 0;
+        uint32_t some = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (x[e] >= least) {
+                sum += x[e];
+                some++;
+            }
+        const Pair total{warp_add(sum), __reduce_add_sync(FULL_MASK, some)};
+        __syncthreads();
         const u64 target = share(m, total.a, false);
         u64 upto = 0;  // kept weight of the lower ids
 #pragma unroll 8
@@ -714,14 +742,18 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) k_sample(SampleArgs a, int sli
         const int wanted = k <= GROUPS / 2 ? k : int(ceilf(GROUPS * (1.f - __expf(-(1.25f * k + 24.f) / GROUPS))));
         const int j = max(min(wanted, some), 1);
         // the j-th largest of the groups' maxima: a quarter of them for each of four threads to compare with
-        const int i = t / 4;
-        int above = 0;
+        const float own = shared.tops[t / 4];
+        int above = 0, no_less = 0;
 #pragma unroll 8
-        for (int o = t & 3; o < GROUPS; o += 4)
-            above += shared.tops[o] > shared.tops[i] || (shared.tops[o] == shared.tops[i] && o < i);
+        for (int o = t & 3; o < GROUPS; o += 4) {
+            above += shared.tops[o] > own;
+            no_less += shared.tops[o] >= own;
+        }
         above += __shfl_xor_sync(FULL_MASK, above, 1);
+        no_less += __shfl_xor_sync(FULL_MASK, no_less, 1);
         above += __shfl_xor_sync(FULL_MASK, above, 2);
-        if (above == j - 1) shared.least_top = shared.tops[i];
+        no_less += __shfl_xor_sync(FULL_MASK, no_less, 2);
+        if (above < j && j <= no_less) shared.least_top = own;  // equal maxima write the same
         __syncthreads();
         const float from = shared.least_top;
         const int n = row.gather(from, far);
@@ -865,7 +897,7 @@ template <int TYPE>
 cudaError_t launch(const SampleArgs& a, cudaStream_t s) {
     constexpr int SIZE = TYPE == 2 ? 4 : 2, VEC = 16 / SIZE;
     // blocks a row: enough that two blocks' slices fit an SM, and more while every block still has an SM of its own (32
-    // rows of 107,520 by top-k: 11.6 us on 4 blocks a row, 16.9 us on 8, which share SMs)
+    // rows of 107,520 by top-k: 11.0 us on 4 blocks a row, 5 more on 8, which share SMs)
     int ranks = 1;
     while (ranks < MAX_CLUSTER && a.vocab / ranks > 2048 &&
            ((long long)a.vocab * SIZE > (long long)ranks * (SLICE_BYTES / 4 * 3) || a.rows * ranks <= 74))
