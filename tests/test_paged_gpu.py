@@ -445,6 +445,19 @@ def test_attention_tiny_probabilities_add_up(torch, pkg):
         assert (np.abs(lse[0] - l) <= 2.0 ** -16).all()
 
 
+@pytest.mark.parametrize("dtype,head_dim", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("requests", [2, 10, 25, 50, 90])
+def test_attention_cut_requests(torch, pkg, requests, dtype, head_dim):
+    """Long requests beside none, one and a few keys: every number of pieces a head, every size of cluster."""
+    rng = np.random.default_rng(requests)
+    for longest in (700, 2500, 9000):
+        lens = rng.integers(longest // 2, longest + 1, requests)
+        lens[:requests // 5] = rng.integers(0, 40, requests // 5)
+        lens[-1] = longest
+        c = Case(torch, pkg.runtime, list(map(int, rng.permutation(lens))), 5, 1, head_dim, 16, dtype=dtype)
+        c.check(*c.run())
+
+
 def test_attention_offsets_past_32_bits(torch, pkg):
     """Three pages 2^30 + 8 elements apart: byte and element offsets pass 2^31 and 2^32."""
     rt, step = pkg.runtime, (1 << 30) + 8
@@ -563,6 +576,25 @@ def test_sample_unusual_distributions(torch, pkg, dtype, vocab, shape):
             sample_check(seen[r], ids[r], lp[r], kept[r], 0.9, k, p, mp, u[r])
             if p == 1.0 and k:
                 assert kept[r] == k
+
+
+@pytest.mark.parametrize("heads", [(1, 2, 63, 64), (65, 127, 128, 129), (1023, 1024, 1025, 1030), (4000, 500, 9000, 8191)])
+@pytest.mark.parametrize("dtype,vocab", [("bf16", 9003), ("f32", 120001)])
+def test_sample_few_and_many_within_reach(torch, pkg, dtype, vocab, heads):
+    """All but a row's `heads` values are too unlikely to weigh anything; those lie next to each other or anywhere."""
+    rng, rows = np.random.default_rng(sum(heads)), 2 * len(heads)
+    x = np.full((rows, vocab), -60.0)
+    for r in range(rows):
+        n = heads[r // 2]
+        at = rng.permutation(vocab)[:n] if r % 2 else (vocab - n) // 3 + np.arange(n)
+        x[r, at] = 1.5 * rng.standard_normal(n)
+    for k, p, mp in ((0, 1.0, 0.0), (0, 0.9, 0.0), (60, 1.0, 0.0), (100, 0.8, 0.0), (128, 0.95, 0.02), (200, 0.5, 0.1), (0, 0.999, 0.0)):
+        u = rng.random(rows).astype(np.float32)
+        ids, lp, kept, seen = run_sample(torch, pkg.runtime, x, dtype, 0.8, k, p, mp, u)
+        for r in range(rows):
+            sample_check(seen[r], ids[r], lp[r], kept[r], 0.8, k, p, mp, u[r])
+            if p == 1.0 and mp == 0.0:
+                assert kept[r] == min(k or vocab, heads[r // 2])
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
