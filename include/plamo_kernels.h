@@ -177,6 +177,8 @@ PLAMO_API int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv,
  * plamo_k_paged_plan), and requests without a token are skipped. heads: a multiple of kv_heads, at most 256.
  *   out = sum_j softmax_j(scale * q.k_j) v_j (scale > 0) in fp32 (the probabilities enter the products as hi + lo pairs
  *   of the 16-bit type), rounded once; lse (may be NULL, [q_rows][heads] fp32) = ln sum_j exp(scale * q.k_j).
+ * An infinite value of a visible key makes its output that infinity, as long as the key's probability is at least 2^-126
+ * of the request's largest (below, fp32 holds no probability: NaN).
  * A request that sees no key, or whose scores are all -inf, gets zeros and lse -inf. Query rows that belong
  * to no request are not written. `workspace`: 16-byte aligned device memory of at least
  * plamo_k_paged_attention_workspace() bytes, no initial contents needed; calls that share one must not

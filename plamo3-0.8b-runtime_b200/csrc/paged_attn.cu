@@ -86,24 +86,28 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid
 }
 
 // Probabilities enter the products as two 16-bit values, hi (cut off, not rounded) and lo = the rest +
-// 2^-16 p: together p (1 + 2^-16) to 15 bits or more, a factor that P_PAIR takes out of the sum. Neither part
-// of a p > 0 is zero or negative, so an infinite value times the pair is that infinity, never inf - inf or 0 inf.
+// 2^-16 p: together p (1 + 2^-16) to 15 bits or more, a factor that P_PAIR takes out of the sum. Neither part of a
+// p > 0 is negative, and neither may vanish, so an infinite value times the pair is that infinity, never inf - inf
+// or 0 inf: a part that has rounded to zero is raised to the least the type holds (fp16: 2^-24, by P_SHIFT 2^-38 of the
+// largest probability; bf16: 2^-126, its least normal number). p itself is zero below 2^-126 of the largest.
 constexpr float P_PAIR = 1.0f + 1.0f / 65536.0f;
 template <bool HALF>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
     constexpr float EXTRA = 1.0f / 65536.0f;
+    const uint32_t bx = __float_as_uint(x), by = __float_as_uint(y), cut = prmt(bx, by, 0x7632);
+    // positive 16-bit floats order as whole numbers do; the upper half of an fp32 p is zero for p = 0 alone
+    const uint32_t least = __vminu2(cut, HALF ? 0x00010001u : 0x00800080u);
     if (HALF) {
         const __half2 h = __halves2half2(__float2half_rz(x), __float2half_rz(y));
         const float2 f = __half22float2(h);
         const __half2 l = __floats2half2_rn(fmaf(x, EXTRA, x - f.x), fmaf(y, EXTRA, y - f.y));
-        hi = *reinterpret_cast<const uint32_t*>(&h);
-        lo = *reinterpret_cast<const uint32_t*>(&l);
+        hi = __vmaxu2(*reinterpret_cast<const uint32_t*>(&h), least);
+        lo = __vmaxu2(*reinterpret_cast<const uint32_t*>(&l), least);
     } else {
-        const uint32_t bx = __float_as_uint(x), by = __float_as_uint(y);
-        hi = prmt(bx, by, 0x7632);
+        hi = cut;
         const __nv_bfloat162 l = __floats2bfloat162_rn(fmaf(x, EXTRA, x - __uint_as_float(bx & 0xffff0000u)),
                                                        fmaf(y, EXTRA, y - __uint_as_float(by & 0xffff0000u)));
-        lo = *reinterpret_cast<const uint32_t*>(&l);
+        lo = __vmaxu2(*reinterpret_cast<const uint32_t*>(&l), least);
     }
 }
 template <bool HALF>
