@@ -245,6 +245,7 @@ __device__ __forceinline__ void add_tile(Running<D>& run, const uint32_t (&qa)[D
 // Four finished outputs of a head, and its lse.
 template <bool HALF>
 __device__ __forceinline__ void store_row(const PagedAttnArgs& a, int qrow, int head, int D, int d, float4 o, float m, float l) {
+    if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);  // no score above -inf: zeros, whatever the values made of 0 p
     const float inv = 1.0f / (l > 0.f ? l * P_PAIR : 1.f);
     uint2 w;
     w.x = round16<HALF>(o.x * inv) | uint32_t(round16<HALF>(o.y * inv)) << 16;
