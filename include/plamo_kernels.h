@@ -139,7 +139,8 @@ typedef struct plamo_paged_cache {
  * 1...8192) holds the first ceil(lens[r] / page_size) entries of its row of table [rows][table_stride].
  *   append[r] >= 0: the step appends that many tokens to it; append[r] < 0: the request has ended.
  * Ended requests' pages go onto the end of free_list (capacity `pages` entries, the first *free_count of
- * them valid), in request order; the pages the appended tokens need then come off its end, in request
+ * them valid), in request order; entries outside [0, pages), of pages given up before, are no pages and are passed
+ * over. The pages the appended tokens need then come off its end, in request
  * order, as long as they last: a request is refused (nothing granted, nothing appended) when the pages
  * needed up to and including it exceed the free ones, when it would outgrow its table row, or when its
  * tokens pass the `tokens` capacity. Outputs: the granted pages in table; new_lens[r] (0 for an ended
