@@ -6,7 +6,8 @@ A step takes the next tokens of every running request (a whole prompt, or the id
 with the kernel-level entry points (include/plamo_kernels.h): one plan gives the tokens their pages and slots,
 every layer appends its keys and values to its own cache by the same slots and attends over the pages, and the last
 hidden row of every request becomes an id by its own controls. Requests come and go between steps; the pages of an
-ended one return to the free list in the plan of the step after. Nothing but the ids leaves the device.
+ended one return to the free list in the plan of the step after. Only the ids and the number of refused requests
+leave the device.
 
 Without --model, a small synthetic model is written to a temporary directory.
 """
@@ -153,7 +154,19 @@ class Engine:
 
 def serve(engine, prompts, new_tokens, controls=None, on_step=None):
     """Runs every prompt to new_tokens ids, as many at a time as the engine has rows. Returns the ids by prompt.
-    controls: (temperature, top_k, top_p, min_p) by prompt. on_step(engine, running): called after every step."""
+    controls: (temperature, top_k, top_p, min_p) by prompt. on_step(engine, running): called after every step.
+    ValueError for a prompt that no step could take: an empty one, one longer than a step has room for beside a token
+    of every other row, one that outgrows the context."""
+    room = engine.tokens - engine.rows
+    if new_tokens < 1:
+        raise ValueError(f"new_tokens is {new_tokens}, at least 1 is needed")
+    for i, prompt in enumerate(prompts):
+        if not len(prompt):
+            raise ValueError(f"prompt {i} is empty")
+        if len(prompt) > room:
+            raise ValueError(f"prompt {i} has {len(prompt)} ids, a step takes at most {room}")
+        if len(prompt) + new_tokens - 1 > engine.context:
+            raise ValueError(f"prompt {i} with {new_tokens} new ids outgrows the context of {engine.context}")
     waiting, running, answers = list(range(len(prompts))), [None] * engine.rows, [[] for _ in prompts]
     ended = [False] * engine.rows
     while waiting or any(r is not None for r in running):
