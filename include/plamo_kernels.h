@@ -148,8 +148,8 @@ typedef struct plamo_paged_cache {
  * step's tokens are packed in request order); for each of `tokens` packed tokens its position and its slot
  * (page * page_size + offset), both -1 for a refused request's tokens and past the last token; counts[4]:
  * free pages left (the next step's free_count), tokens, pages granted, requests refused. An ended
- * request's table row is left as it was. Entries outside [0, pages) give slot -1. Outputs must not overlap
- * inputs, except that table and free_list are updated in place. All values int32. */
+ * request's table row is left as it was. Entries outside [0, pages) give slot -1. table and free_list are
+ * updated in place; no array that is written may overlap another one. All values int32. */
 PLAMO_API int plamo_k_paged_plan(const int32_t* lens, const int32_t* append, int rows, int page_size, int pages,
                                  int32_t* table, int table_stride, int32_t* free_list, const int32_t* free_count,
                                  int32_t* new_lens, int32_t* row_start, int32_t* slots, int32_t* positions, int tokens,

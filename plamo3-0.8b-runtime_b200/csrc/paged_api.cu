@@ -25,6 +25,16 @@ int invalid(const char* what, const char* more = "") {
 int launched(cudaError_t e) { return e == cudaSuccess ? 0 : invalid("CUDA error: ", cudaGetErrorString(e)); }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// The bytes of an array of n 32-bit values.
+struct Range {
+    uintptr_t begin, end;
+};
+Range range(const int32_t* p, long long n) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return {at, at + uintptr_t(n) * 4};
+}
+bool overlap(const Range& x, const Range& y) { return x.begin < y.end && y.begin < x.end; }
+
 // Null, or the words that say what is wrong with a cache descriptor.
 const char* cache_fault(const plamo_paged_cache* c) {
     if (!c || !c->keys || !c->values) return "Invalid paged cache";
@@ -55,8 +65,16 @@ int plamo_k_paged_plan(const int32_t* lens, const int32_t* append, int rows, int
         tokens > INT_MAX - 64 * PAGED_MAX_ROWS || (long long)pages * page_size > INT_MAX ||
         (long long)rows * table_stride > INT_MAX)
         return invalid("Invalid paged plan arguments");
-    if (new_lens == lens || new_lens == append || counts == free_count)
-        return invalid("A paged plan's outputs must not overlap its inputs");
+    // every array that is written, table and free_list among them, lies apart from every other one
+    const Range written[] = {range(table, (long long)rows * table_stride), range(free_list, pages), range(new_lens, rows),
+                             range(row_start, rows + 1ll), range(slots, tokens), range(positions, tokens), range(counts, 4)};
+    const Range read[] = {range(lens, rows), range(append, rows), range(free_count, 1)};
+    for (const Range& w : written) {
+        for (const Range& r : read)
+            if (overlap(w, r)) return invalid("A paged plan's outputs must not overlap its inputs");
+        for (const Range& o : written)
+            if (&o != &w && overlap(w, o)) return invalid("A paged plan's outputs must not overlap each other");
+    }
     return launched(launch_paged_plan({lens, append, rows, page_size, pages, table, table_stride, free_list, free_count,
                                        new_lens, row_start, slots, positions, tokens, counts},
                                       static_cast<cudaStream_t>(stream)));
