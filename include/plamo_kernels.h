@@ -117,7 +117,7 @@ PLAMO_API int plamo_k_exp(const float* x, float* y, long long n, void* stream);
  * One step of a changing set of requests is
  *     plamo_k_paged_plan -> per layer: plamo_k_paged_qkv, plamo_k_paged_attention -> plamo_k_sample
  * All four enqueue on `stream`, allocate nothing, keep nothing between calls and can be captured in a
- * CUDA graph. Values are bf16 (dtype 0) or fp16 (dtype 1) bit patterns. */
+ * CUDA graph. Values are bf16 (dtype 0) or fp16 (dtype 1) bit patterns. Arrays of 32-bit values are 4-byte aligned. */
 
 /* One layer's paged cache. The value of token slot t = page * page_size + offset, KV head h, element d
  * is at keys[page * page_stride + offset * token_stride + h * head_stride + d] (values alike); strides in

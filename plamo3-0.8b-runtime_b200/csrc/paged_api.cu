@@ -5,6 +5,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 #include <string>
 
 namespace plamo {
@@ -24,6 +25,13 @@ int invalid(const char* what, const char* more = "") {
 }
 int launched(cudaError_t e) { return e == cudaSuccess ? 0 : invalid("CUDA error: ", cudaGetErrorString(e)); }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Whether arrays of 32-bit values (null ones aside) lie on 4-byte boundaries.
+bool aligned4(std::initializer_list<const void*> arrays) {
+    for (const void* p : arrays)
+        if (reinterpret_cast<uintptr_t>(p) & 3) return false;
+    return true;
+}
+constexpr const char* MISALIGNED = "Arrays of 32-bit values must be 4-byte aligned";
 
 // The bytes of an array of n 32-bit values.
 struct Range {
@@ -65,6 +73,8 @@ int plamo_k_paged_plan(const int32_t* lens, const int32_t* append, int rows, int
         tokens > INT_MAX - 64 * PAGED_MAX_ROWS || (long long)pages * page_size > INT_MAX ||
         (long long)rows * table_stride > INT_MAX)
         return invalid("Invalid paged plan arguments");
+    if (!aligned4({lens, append, table, free_list, free_count, new_lens, row_start, slots, positions, counts}))
+        return invalid(MISALIGNED);
     // every array that is written, table and free_list among them, lies apart from every other one
     const Range written[] = {range(table, (long long)rows * table_stride), range(free_list, pages), range(new_lens, rows),
                              range(row_start, rows + 1ll), range(slots, tokens), range(positions, tokens), range(counts, 4)};
@@ -90,6 +100,7 @@ int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv, int64_t q
         !(eps >= 0.f))
         return invalid("Invalid paged qkv arguments");
     if ((long long)tokens * (heads + 2 * cache->kv_heads) > INT_MAX / 2) return invalid("Too many tokens in one paged qkv call");
+    if (!aligned4({positions, slots})) return invalid(MISALIGNED);
     if (!aligned16(qkv) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(rope) || !aligned16(q))
         return invalid("Paged qkv pointers must be 16-byte aligned");
     return launched(launch_paged_qkv({cache_args(cache), static_cast<const uint16_t*>(qkv), qkv_stride, tokens, heads,
@@ -111,6 +122,7 @@ int plamo_k_paged_attention(const plamo_paged_cache* cache, const void* q, int64
         q_stride < (long long)heads * cache->head_dim || out_stride < (long long)heads * cache->head_dim || q_stride % 8 ||
         out_stride % 8)
         return invalid("Invalid paged attention arguments");
+    if (!aligned4({table, lens, row_start, lse})) return invalid(MISALIGNED);
     if (!aligned16(q) || !aligned16(out)) return invalid("Paged attention pointers must be 16-byte aligned");
     if (!workspace || !aligned16(workspace) || workspace_bytes < paged_attention_workspace()) {
         char words[96];
@@ -130,6 +142,7 @@ int plamo_k_sample(const void* logits, int dtype, int rows, int vocab, int64_t r
     if (!logits || !u || !ids || dtype < 0 || dtype > 2 || rows < 1 || rows > 65535 || vocab < 1 ||
         vocab > SAMPLE_MAX_VOCAB || row_stride < vocab || (reinterpret_cast<uintptr_t>(logits) & (dtype == 2 ? 3 : 1)))
         return invalid("Invalid sample arguments");
+    if (!aligned4({temperature, top_k, top_p, min_p, u, ids, logprobs, kept})) return invalid(MISALIGNED);
     return launched(launch_sample({logits, rows, vocab, row_stride, temperature, top_k, top_p, min_p, u, ids, logprobs, kept},
                                   dtype, static_cast<cudaStream_t>(stream)));
 }
