@@ -172,7 +172,8 @@ PLAMO_API int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv,
 /* Attention of one new token of every request over its pages. Request r (of rows, 1...8192) sees the keys
  * at positions [max(0, n - window), n), n = min(lens[r], max_len) (window 0: all of them); the key at
  * position p is in page table[r][p / page_size]; entries outside [0, pages) hold no keys (a page given up
- * behind the window). max_len bounds the lengths for the launch: at most table_stride * page_size.
+ * behind the window). max_len bounds the lengths for the launch: at most table_stride * page_size. How the work is split
+ * is chosen by it, so short requests run faster under a bound near their longest.
  * row_start NULL: request r's query is row r of q [q_rows][heads][head_dim] (q_stride elements apart), and
  * q_rows >= rows. Else it is row row_start[r + 1] - 1 (the request's last packed token of
  * plamo_k_paged_plan), and requests without a token are skipped. heads: a multiple of kv_heads, at most 256.
