@@ -184,7 +184,8 @@ PLAMO_API int plamo_k_paged_qkv(const plamo_paged_cache* cache, const void* qkv,
  * A request that sees no key, or whose scores are all -inf, gets zeros and lse -inf. Query rows that belong
  * to no request are not written. `workspace`: 16-byte aligned device memory of at least
  * plamo_k_paged_attention_workspace() bytes, no initial contents needed; calls that share one must not
- * overlap. Pointers 16-byte aligned, strides multiples of 8. */
+ * overlap. out, lse and workspace lie apart from each other and from every input. Pointers 16-byte aligned, strides
+ * multiples of 8. */
 PLAMO_API int plamo_k_paged_attention(const plamo_paged_cache* cache, const void* q, int64_t q_stride, int q_rows, int heads,
                                       const int32_t* table, int table_stride, const int32_t* lens, int rows,
                                       const int32_t* row_start, int max_len, int window, float scale, void* out,
@@ -205,7 +206,7 @@ PLAMO_API size_t plamo_k_paged_attention_workspace(void);
  * id is the lowest kept index at which the running sum of kept w exceeds floor(2^24 u) * W / 2^24, W the
  * sum of all kept w. ids[row]; logprobs[row] (may be NULL) = ln(w_id / W); kept[row] (may be NULL) the number
  * of kept ids. NaN and -inf logits are never chosen; a row of only those gives id 0, logprob -inf and kept 0.
- * Equal +inf logits share the probability. */
+ * Equal +inf logits share the probability. ids, logprobs and kept lie apart from each other and from every input. */
 PLAMO_API int plamo_k_sample(const void* logits, int dtype, int rows, int vocab, int64_t row_stride,
                              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                              const float* u, int32_t* ids, float* logprobs, int32_t* kept, void* stream);
